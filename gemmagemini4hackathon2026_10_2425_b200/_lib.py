@@ -16,6 +16,7 @@ HEADER = Path(__file__).resolve().parents[1] / "include" / "b200dec.h"
 OK, ERR_NULL, ERR_SHAPE, ERR_ALIGN, ERR_UNSUPPORTED, ERR_WORKSPACE = 0, 1, 2, 3, 4, 5
 ERR_CUDA, ERR_NCCL, ERR_TIMEOUT, ERR_STATE = 6, 7, 8, 9
 F32, F16, Q8_32, Q4_32, F16X2 = 0, 1, 2, 3, 4
+PLAN_OK, PLAN_PAGES, PLAN_TABLE, PLAN_ROWS, PLAN_TREE = 0, 1, 2, 3, 4
 EPI_STORE, EPI_ADD, EPI_GELU_MUL, EPI_SWIGLU, EPI_ARGMAX, EPI_SILU_MUL = 0, 1, 2, 3, 4, 5
 
 P = C.c_void_p
@@ -91,6 +92,15 @@ SIGNATURES = {
         I,
         [P, I, I, P, P, P, I, I, P, P, I, I, I, I, I, Fl, I, I, P, I, I, P],
     ),
+    "b2d_paged_plan": (I, [P, P, P, P, I, P, P, I, P, I, I, I, P, P, P, P, P, P, P, P]),
+    "b2d_qk_norm_rope_append": (I, [P, I, I, P, P, Fl, I, P, P, P, P, P, I, I, P, P, I, I, I, I, I, P]),
+    "b2d_paged_tree_attn_workspace_bytes": (Z, [I, I, I, I, I, I, I]),
+    "b2d_paged_tree_attn_error": (I, []),
+    "b2d_paged_tree_attn": (
+        I,
+        [P, I, I, P, P, P, I, I, P, P, P, I, P, I, I, I, I, I, I, I, Fl, I, P, I, I, P, Z, P],
+    ),
+    "b2d_token_logprobs": (I, [P, I, C.c_longlong, I, I, P, P, I, I, P, P, P, P, P]),
     "b2d_nccl_unique_id_bytes": (I, []),
     "b2d_nccl_get_unique_id": (I, [P]),
     "b2d_decoder_create": (I, [C.POINTER(ModelConfig), I, I, P, C.POINTER(P)]),

@@ -68,6 +68,20 @@ int paged_decode_attn(void*, int, int, uint16_t*, uint16_t*, const int*, int, in
                       const float*, int, int, int, int, int, float, int, int, void*, int, int,
                       void*, size_t, cudaStream_t);
 
+// plan.cu / qk_append.cu / tree_attn.cu / logprobs.cu
+int paged_plan(const int*, const int*, const int*, int*, int, const int*, int*, int, const int*, int,
+               int, int, int*, long long*, int*, uint32_t*, int*, int*, int*, cudaStream_t);
+int qk_norm_rope_append(const void*, int, int, const float*, const float*, float, int, const int*,
+                        const long long*, const int*, const float*, void*, int, int, uint16_t*,
+                        uint16_t*, int, int, int, int, int, cudaStream_t);
+size_t paged_tree_attn_workspace_bytes(int, int, int, int, int, int, int);
+int paged_tree_attn_error();
+int paged_tree_attn(const void*, int, int, const uint16_t*, const uint16_t*, const int*, int, int,
+                    const int*, const int*, const uint32_t*, int, const int*, int, int, int, int,
+                    int, int, int, float, int, void*, int, int, void*, size_t, cudaStream_t);
+int token_logprobs(const void*, int, long long, int, int, const int*, const int*, int, int, float*,
+                   float*, int*, float*, cudaStream_t);
+
 }  // namespace b2d
 
 using namespace b2d;
@@ -298,6 +312,55 @@ int b2d_paged_decode_attn(void* qkv, int qkv_dtype, int ldqkv, uint16_t* k_pages
                            n_blocks, ctx_lens, inv_freq, n_heads, n_kv_heads, head_dim, batch,
                            max_ctx, scale, window, append, out, out_dtype, ldout, workspace,
                            workspace_bytes, S(stream));
+}
+
+int b2d_paged_plan(const int* ctx_lens, const int* q_lens, const int* parents, int* block_table,
+                   int max_blocks, const int* n_pages, int* free_pages, int free_capacity,
+                   const int* n_free, int batch, int max_tokens, int mask_words, int* cu_q,
+                   long long* slots, int* positions, uint32_t* mask, int* status, int* n_pages_out,
+                   int* n_free_out, b2d_stream_t stream) {
+  return paged_plan(ctx_lens, q_lens, parents, block_table, max_blocks, n_pages, free_pages,
+                    free_capacity, n_free, batch, max_tokens, mask_words, cu_q, slots, positions,
+                    mask, status, n_pages_out, n_free_out, S(stream));
+}
+
+int b2d_qk_norm_rope_append(const void* qkv, int qkv_dtype, int ldqkv, const float* q_gamma,
+                            const float* k_gamma, float eps, int v_norm, const int* positions,
+                            const long long* slots, const int* n_rows, const float* inv_freq,
+                            void* q_out, int q_dtype, int ldq, uint16_t* k_pages,
+                            uint16_t* v_pages, int n_blocks, int n_heads, int n_kv_heads,
+                            int head_dim, int rows, b2d_stream_t stream) {
+  return qk_norm_rope_append(qkv, qkv_dtype, ldqkv, q_gamma, k_gamma, eps, v_norm, positions, slots,
+                             n_rows, inv_freq, q_out, q_dtype, ldq, k_pages, v_pages, n_blocks,
+                             n_heads, n_kv_heads, head_dim, rows, S(stream));
+}
+
+size_t b2d_paged_tree_attn_workspace_bytes(int batch, int rows, int n_heads, int n_kv_heads,
+                                           int head_dim, int max_q, int max_ctx) {
+  return paged_tree_attn_workspace_bytes(batch, rows, n_heads, n_kv_heads, head_dim, max_q, max_ctx);
+}
+
+int b2d_paged_tree_attn_error(void) { return paged_tree_attn_error(); }
+
+int b2d_paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages,
+                        const uint16_t* v_pages, const int* block_table, int max_blocks,
+                        int n_blocks, const int* ctx_lens, const int* cu_q, const uint32_t* mask,
+                        int mask_words, const int* positions, int n_heads, int n_kv_heads,
+                        int head_dim, int batch, int rows, int max_q, int max_ctx, float scale,
+                        int window, void* out, int out_dtype, int ldout, void* workspace,
+                        size_t workspace_bytes, b2d_stream_t stream) {
+  return paged_tree_attn(q, q_dtype, ldq, k_pages, v_pages, block_table, max_blocks, n_blocks,
+                         ctx_lens, cu_q, mask, mask_words, positions, n_heads, n_kv_heads, head_dim,
+                         batch, rows, max_q, max_ctx, scale, window, out, out_dtype, ldout,
+                         workspace, workspace_bytes, S(stream));
+}
+
+int b2d_token_logprobs(const void* logits, int dtype, long long ld, int V, int rows,
+                       const int* n_rows, const int* targets, int n_targets, int top_k,
+                       float* logprobs, float* entropy, int* top_ids, float* top_logprobs,
+                       b2d_stream_t stream) {
+  return token_logprobs(logits, dtype, ld, V, rows, n_rows, targets, n_targets, top_k, logprobs,
+                        entropy, top_ids, top_logprobs, S(stream));
 }
 
 }  // extern "C"

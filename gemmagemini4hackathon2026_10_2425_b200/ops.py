@@ -9,6 +9,10 @@ Reference mapping (LK = ios_kernels/kernels/unsloth__Llama-3.2-1B-Instruct/
 kernel_metal_f16_20261024-1620): gemv* <- matvec_f16 / matvec_gate_up_silu
 (LK/kernels.metal:106-173), rmsnorm <- LK/kernels.metal:71-89, paged_decode_attn <-
 attention + rope_kv (LK/kernels.metal:182-305), lm_head_argmax <- argmax (:307-345).
+
+A step with several rows per sequence (drafted tokens, prompt chunks) is paged_plan, then per layer
+qk_norm_rope_append and paged_tree_attn, then token_logprobs.  These four run on the device and the
+current stream of their tensors' device, keep nothing between calls and use no shared workspace.
 """
 
 from __future__ import annotations
@@ -620,5 +624,375 @@ def add_rmsnorm_f16(x: torch.Tensor, gamma: torch.Tensor, eps: float, p: torch.T
     call(
         "b2d_add_rmsnorm", x.data_ptr(), _ptr(p), gamma.data_ptr(), float(eps), _lib.F16X2 if x2 else _lib.F16,
         out.data_ptr(), x.shape[0], x.shape[1], _stream(),
+    )
+    return out
+
+
+# -- several rows per sequence: drafted tokens and prompt chunks ---------------------------------
+
+
+def _check(name: str, t: torch.Tensor | None, dtypes, dev: torch.device, shape=None, rows: bool = False) -> None:
+    """t (None passes) is on dev, of one of dtypes and of `shape` (None entries are free), contiguous
+    (with rows: only each row is, at any row stride)."""
+    if t is None:
+        return
+    if not t.is_cuda or t.device != dev:
+        raise ValueError(f"{name} must be a CUDA tensor on {dev} (no CPU path exists)")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} has dtype {t.dtype}, expected one of {[str(d) for d in dtypes]}")
+    if shape is not None and (t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape))):
+        raise ValueError(f"{name} has shape {list(t.shape)}, expected {list(shape)}")
+    if rows:
+        if t.stride(-1) != 1 and t.shape[-1] > 1 or t.dim() == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+            raise ValueError(f"{name} needs contiguous rows that do not overlap")
+    elif not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row stride of a [rows, n] tensor whose rows do not overlap."""
+    return max(t.stride(0), t.shape[1])
+
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """call() with the current stream of dev as the last argument, on dev."""
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if dev.index == torch.cuda.current_device():
+        call(name, *args, stream)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, stream)
+
+
+_I32, _I64, _F32, _F16 = (torch.int32,), (torch.int64,), (torch.float32,), (torch.float16,)
+_FLOATS = (torch.float32, torch.float16)
+
+
+@dataclass
+class PagedPlan:
+    """paged_plan()'s outputs for a batch of B requests and R rows.  Rows from cu_q[B] on belong to no
+    request and are left as they were."""
+
+    cu_q: torch.Tensor  # int32 [B + 1]: first row of each request, then their total
+    slots: torch.Tensor  # int64 [R]: page * 16 + place in the page, -1 for none
+    positions: torch.Tensor  # int32 [R]
+    mask: torch.Tensor | None  # int32 [R, words]: bit j = row j of the request is an ancestor, or the row itself
+    status: torch.Tensor  # int32 [B]: _lib.PLAN_OK, PLAN_PAGES, PLAN_TABLE, PLAN_ROWS or PLAN_TREE
+    n_pages: torch.Tensor  # int32 [B]: pages each request has now
+    n_free: torch.Tensor  # int32 [1]: pages left on the free stack
+
+    @property
+    def n_rows(self) -> torch.Tensor:
+        """int32 [1], on the device: the number of rows in use (qk_norm_rope_append's n_rows)."""
+        return self.cu_q[-1:]
+
+
+def paged_plan(
+    ctx_lens: torch.Tensor,
+    q_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    n_pages: torch.Tensor,
+    free_pages: torch.Tensor,
+    n_free: torch.Tensor,
+    max_tokens: int,
+    *,
+    parents: torch.Tensor | None = None,
+    mask_words: int = 0,
+    out: PagedPlan | None = None,
+) -> PagedPlan:
+    """Pages, slots, positions and tree masks of a step that adds q_lens[b] rows to request b (a
+    negative number ends it and gives its pages back); block_table and free_pages are updated in
+    place, n_pages and n_free if `out` holds them.  See include/b200dec.h b2d_paged_plan.  ctx_lens,
+    q_lens, n_pages int32 [B]; block_table int32 [B, max_blocks]; free_pages int32 [capacity]; n_free
+    int32 [1]; parents int32 [max_tokens] with mask_words (<= 8) words of 32 nodes per row."""
+    dev = ctx_lens.device
+    B = ctx_lens.numel()
+    _check("ctx_lens", ctx_lens, _I32, dev, (B,))
+    _check("q_lens", q_lens, _I32, dev, (B,))
+    _check("block_table", block_table, _I32, dev, (B, None))
+    _check("n_pages", n_pages, _I32, dev, (B,))
+    _check("free_pages", free_pages, _I32, dev, (None,))
+    _check("n_free", n_free, _I32, dev, (1,))
+    _check("parents", parents, _I32, dev, (max_tokens,))
+    if (parents is None) != (mask_words == 0):
+        raise ValueError("parents and mask_words go together")
+    if out is None:
+        i32 = dict(dtype=torch.int32, device=dev)
+        out = PagedPlan(
+            torch.empty(B + 1, **i32),
+            torch.empty(max_tokens, dtype=torch.int64, device=dev),
+            torch.empty(max_tokens, **i32),
+            torch.empty(max_tokens, mask_words, **i32) if mask_words else None,
+            torch.empty(B, **i32),
+            torch.empty(B, **i32),
+            torch.empty(1, **i32),
+        )
+    else:
+        _check("out.cu_q", out.cu_q, _I32, dev, (B + 1,))
+        _check("out.slots", out.slots, _I64, dev, (max_tokens,))
+        _check("out.positions", out.positions, _I32, dev, (max_tokens,))
+        _check("out.status", out.status, _I32, dev, (B,))
+        _check("out.n_pages", out.n_pages, _I32, dev, (B,))
+        _check("out.n_free", out.n_free, _I32, dev, (1,))
+        if mask_words:
+            if out.mask is None:
+                raise ValueError("out.mask is missing")
+            _check("out.mask", out.mask, _I32, dev, (max_tokens, mask_words))
+    _call_on(
+        dev,
+        "b2d_paged_plan",
+        ctx_lens.data_ptr(),
+        q_lens.data_ptr(),
+        _ptr(parents),
+        block_table.data_ptr(),
+        block_table.shape[1],
+        n_pages.data_ptr(),
+        free_pages.data_ptr(),
+        free_pages.numel(),
+        n_free.data_ptr(),
+        B,
+        max_tokens,
+        mask_words,
+        out.cu_q.data_ptr(),
+        out.slots.data_ptr(),
+        out.positions.data_ptr(),
+        out.mask.data_ptr() if mask_words else None,
+        out.status.data_ptr(),
+        out.n_pages.data_ptr(),
+        out.n_free.data_ptr(),
+    )
+    return out
+
+
+def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, n_kv_heads: int, head_dim: int, dev: torch.device) -> None:
+    _check("k_pages", k_pages, _F16, dev, (None, n_kv_heads, 16, head_dim))
+    _check("v_pages", v_pages, _F16, dev, tuple(k_pages.shape))
+
+
+def qk_norm_rope_append(
+    qkv: torch.Tensor,
+    positions: torch.Tensor,
+    slots: torch.Tensor,
+    inv_freq_dev: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    n_heads: int,
+    n_kv_heads: int,
+    head_dim: int,
+    *,
+    q_gamma: torch.Tensor | None = None,
+    k_gamma: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    v_norm: bool = False,
+    n_rows: torch.Tensor | None = None,
+    q_out: torch.Tensor | None = None,
+    out_dtype: torch.dtype = torch.float32,
+) -> torch.Tensor:
+    """Per-head norms of q and k (where a gamma is given), rotation by positions and append of k and
+    v to their slots, for rows of qkv [R, (Hq + 2 Hkv) * HD]; returns the rotated q [R, Hq * HD].
+    See include/b200dec.h b2d_qk_norm_rope_append.  positions int32 [R], slots int64 [R] and n_rows
+    (int32 [1], optional: rows in use) as paged_plan returns them."""
+    dev, R, nq = qkv.device, qkv.shape[0], n_heads * head_dim
+    _check("qkv", qkv, _FLOATS, dev, (R, (n_heads + 2 * n_kv_heads) * head_dim), rows=True)
+    if q_out is None:
+        q_out = torch.empty(R, nq, dtype=out_dtype, device=dev)
+    _check("q_out", q_out, _FLOATS, dev, (R, nq), rows=True)
+    _check("positions", positions, _I32, dev, (R,))
+    _check("slots", slots, _I64, dev, (R,))
+    _check("inv_freq_dev", inv_freq_dev, _F32, dev, (head_dim // 2,))
+    _check("q_gamma", q_gamma, _F32, dev, (head_dim,))
+    _check("k_gamma", k_gamma, _F32, dev, (head_dim,))
+    _check("n_rows", n_rows, _I32, dev, (1,))
+    _check_pages(k_pages, v_pages, n_kv_heads, head_dim, dev)
+    if R == 0:
+        return q_out
+    _call_on(
+        dev,
+        "b2d_qk_norm_rope_append",
+        qkv.data_ptr(),
+        _DT[qkv.dtype],
+        _ld(qkv),
+        _ptr(q_gamma),
+        _ptr(k_gamma),
+        eps,
+        1 if v_norm else 0,
+        positions.data_ptr(),
+        slots.data_ptr(),
+        _ptr(n_rows),
+        inv_freq_dev.data_ptr(),
+        q_out.data_ptr(),
+        _DT[q_out.dtype],
+        _ld(q_out),
+        k_pages.data_ptr(),
+        v_pages.data_ptr(),
+        k_pages.shape[0],
+        n_heads,
+        n_kv_heads,
+        head_dim,
+        R,
+    )
+    return q_out
+
+
+def tree_attn_workspace_bytes(batch, rows, n_heads, n_kv_heads, head_dim, max_q, max_ctx) -> int:
+    return int(
+        _lib.lib().b2d_paged_tree_attn_workspace_bytes(batch, rows, n_heads, n_kv_heads, head_dim, max_q, max_ctx)
+    )
+
+
+def paged_tree_attn(
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    ctx_lens: torch.Tensor,
+    cu_q: torch.Tensor,
+    n_heads: int,
+    n_kv_heads: int,
+    head_dim: int,
+    max_q: int,
+    max_ctx: int,
+    *,
+    mask: torch.Tensor | None = None,
+    positions: torch.Tensor | None = None,
+    scale: float = 0.0,
+    window: int = 0,
+    out: torch.Tensor | None = None,
+    out_dtype: torch.dtype = torch.float32,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of the rows cu_q[b] .. cu_q[b + 1] of each sequence over its ctx_lens[b] cached tokens
+    and, of the step's own rows, those its mask names (mask None: the rows up to itself).  q [R, Hq *
+    HD] is rotated, the rows' k and v are in the cache.  See include/b200dec.h b2d_paged_tree_attn;
+    `out` may be fp16 [2, R, Hq * HD]: the output as B2D_F16X2 hi + lo planes.  The workspace (any
+    contents) is allocated from torch's caching allocator unless given."""
+    dev, R, nq, B = q.device, q.shape[0], n_heads * head_dim, ctx_lens.numel()
+    _check("q", q, _FLOATS, dev, (R, nq), rows=True)
+    if out is None:
+        out = torch.empty(R, nq, dtype=out_dtype, device=dev)
+    x2 = _is_x2(out)
+    if x2:
+        _check("out", out, _F16, dev, (2, R, nq))
+    else:
+        _check("out", out, _FLOATS, dev, (R, nq), rows=True)
+    _check_pages(k_pages, v_pages, n_kv_heads, head_dim, dev)
+    _check("ctx_lens", ctx_lens, _I32, dev, (B,))
+    _check("block_table", block_table, _I32, dev, (B, None))
+    _check("cu_q", cu_q, _I32, dev, (B + 1,))
+    _check("mask", mask, _I32, dev, (R, None))
+    _check("positions", positions, _I32, dev, (R,))
+    if R == 0:
+        return out
+    nbytes = tree_attn_workspace_bytes(B, R, n_heads, n_kv_heads, head_dim, max_q, max_ctx)
+    if workspace is None:
+        if nbytes:
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    else:
+        _check("workspace", workspace, (torch.uint8,), dev, (None,))
+    _call_on(
+        dev,
+        "b2d_paged_tree_attn",
+        q.data_ptr(),
+        _DT[q.dtype],
+        _ld(q),
+        k_pages.data_ptr(),
+        v_pages.data_ptr(),
+        block_table.data_ptr(),
+        block_table.shape[1],
+        k_pages.shape[0],
+        ctx_lens.data_ptr(),
+        cu_q.data_ptr(),
+        _ptr(mask),
+        0 if mask is None else mask.shape[1],
+        _ptr(positions),
+        n_heads,
+        n_kv_heads,
+        head_dim,
+        B,
+        R,
+        max_q,
+        max_ctx,
+        scale,
+        window,
+        out.data_ptr(),
+        _lib.F16X2 if x2 else _DT[out.dtype],
+        nq if x2 else _ld(out),
+        _ptr(workspace),
+        0 if workspace is None else workspace.numel(),
+    )
+    return out
+
+
+def tree_attn_check() -> None:
+    """Synchronize and raise if a bounded wait of a paged_tree_attn call on the current device gave up."""
+    call("b2d_paged_tree_attn_error")
+
+
+@dataclass
+class TokenLogprobs:
+    """token_logprobs()'s outputs for R rows; the fields that were not asked for are None."""
+
+    logprobs: torch.Tensor | None  # fp32, the shape of the targets
+    entropy: torch.Tensor  # fp32 [R], nats
+    top_ids: torch.Tensor | None  # int32 [R, k], falling logits, equal ones by rising index
+    top_logprobs: torch.Tensor | None  # fp32 [R, k]
+
+
+def token_logprobs(
+    logits: torch.Tensor,
+    targets: torch.Tensor | None = None,
+    top_k: int = 0,
+    *,
+    n_rows: torch.Tensor | None = None,
+    out: TokenLogprobs | None = None,
+) -> TokenLogprobs:
+    """Log probabilities of targets (int32 [R] or [R, n]; ids outside the vocabulary: -inf) under the
+    rows of logits [R, V] (fp32 or fp16, any row stride), each row's entropy, and its top_k <= 32 most
+    likely tokens.  See include/b200dec.h b2d_token_logprobs.  Rows from n_rows (int32 [1], on the
+    device) on are skipped: pass `out` to keep what it held there."""
+    dev = logits.device
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, V]")
+    R, V = logits.shape
+    _check("logits", logits, _FLOATS, dev, rows=True)
+    if targets is not None and (targets.dim() not in (1, 2) or targets.shape[0] != R):
+        raise ValueError(f"targets must be int32 [{R}] or [{R}, n]")
+    _check("targets", targets, _I32, dev)
+    _check("n_rows", n_rows, _I32, dev, (1,))
+    f32 = dict(dtype=torch.float32, device=dev)
+    if out is None:
+        out = TokenLogprobs(
+            None if targets is None else torch.empty(targets.shape, **f32),
+            torch.empty(R, **f32),
+            torch.empty(R, top_k, dtype=torch.int32, device=dev) if top_k > 0 else None,
+            torch.empty(R, top_k, **f32) if top_k > 0 else None,
+        )
+    else:
+        if (targets is not None and out.logprobs is None) or (top_k > 0 and (out.top_ids is None or out.top_logprobs is None)):
+            raise ValueError("out lacks a field that was asked for")
+        if targets is not None:
+            _check("out.logprobs", out.logprobs, _F32, dev, tuple(targets.shape))
+        _check("out.entropy", out.entropy, _F32, dev, (R,))
+        if top_k > 0:
+            _check("out.top_ids", out.top_ids, _I32, dev, (R, top_k))
+            _check("out.top_logprobs", out.top_logprobs, _F32, dev, (R, top_k))
+    if R == 0:
+        return out
+    _call_on(
+        dev,
+        "b2d_token_logprobs",
+        logits.data_ptr(),
+        _DT[logits.dtype],
+        _ld(logits),
+        V,
+        R,
+        _ptr(n_rows),
+        _ptr(targets),
+        0 if targets is None else targets.numel() // R,
+        top_k,
+        None if targets is None else out.logprobs.data_ptr(),
+        _ptr(out.entropy),
+        out.top_ids.data_ptr() if top_k > 0 else None,
+        out.top_logprobs.data_ptr() if top_k > 0 else None,
     )
     return out

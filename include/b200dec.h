@@ -323,6 +323,119 @@ B2D_API int b2d_paged_decode_attn_noalloc(void* qkv, int qkv_dtype, int ldqkv, u
                                           int ldout, b2d_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Several rows per sequence: drafted tokens (trees or chains) and prompt chunks of a ragged
+ * batch.  One step is b2d_paged_plan, then per layer b2d_qk_norm_rope_append and
+ * b2d_paged_tree_attn, then b2d_token_logprobs on the logits.  Row r of the step's token buffer
+ * belongs to the request b with cu_q[b] <= r < cu_q[b + 1]; row cu_q[b] + i is stored at place
+ * ctx_lens[b] + i of its cache.  The buffers may be longer than cu_q[batch] (a captured graph's
+ * fixed size): rows behind the last request are neither read nor written.
+ * ------------------------------------------------------------------------------------- */
+
+/* What b2d_paged_plan reports for a request (status[b]). */
+enum b2d_plan_status {
+  B2D_PLAN_OK = 0,
+  B2D_PLAN_PAGES = 1, /* not enough free pages for it, after the requests before it */
+  B2D_PLAN_TABLE = 2, /* more pages than a block-table row holds, or a negative context */
+  B2D_PLAN_ROWS = 3,  /* its rows go past max_tokens (those that fit exist, without slots) */
+  B2D_PLAN_TREE = 4   /* more tree nodes than 32 * mask_words */
+};
+
+/* Pages, slots, positions and tree masks of one step, from the requests' lengths, on the GPU
+ * (engine.make_block_table does the host's part of this).  For each request b of the batch
+ * (<= 8192) with ctx_lens[b] cached tokens and n_pages[b] pages, the entries block_table[b][0 ..
+ * n_pages[b]):
+ *   q_lens[b] >= 0: that many rows are added; pages missing for ctx + q places are popped from
+ *     the free stack free_pages[0 .. *n_free) (its end first, requests in order) and written to
+ *     block_table[b][n_pages[b] ..].  Pages it has beyond that (a rejected draft's) stay its own.
+ *   q_lens[b] < 0: the request ended.  Its pages are pushed onto the stack, before any are popped;
+ *     its block-table row keeps its (now meaningless) entries.
+ * A request that cannot be served keeps its pages and gets status[b] != 0; its rows exist with
+ * slots -1 (b2d_qk_norm_rope_append then stores nothing).  The pages asked for by a refused
+ * request still count against the requests after it, so whether one is served depends on those
+ * before it only.  Outputs: cu_q[batch + 1] (first rows), slots (page * 16 + place in the page,
+ * or -1) and positions per row, n_pages_out[batch] and n_free_out[1] (may be n_pages and n_free),
+ * status[batch].
+ * Without parents, positions are ctx_lens[b] + i.  With parents (int per row: the number, within
+ * the request, of the row a drafted token follows, less than its own; -1, or anything else, the
+ * last cached token) they are ctx_lens[b] + depth, and mask[row][mask_words] (mask_words <= 8)
+ * has bit j set if row j of the request is the row itself or an ancestor of it.
+ * max_tokens <= 2^24 is the size of the row arrays, free_capacity that of free_pages (pages
+ * pushed past it are lost), max_blocks <= 2^17. */
+B2D_API int b2d_paged_plan(const int* ctx_lens, const int* q_lens, const int* parents,
+                           int* block_table, int max_blocks, const int* n_pages, int* free_pages,
+                           int free_capacity, const int* n_free, int batch, int max_tokens,
+                           int mask_words, int* cu_q, long long* slots, int* positions,
+                           uint32_t* mask, int* status, int* n_pages_out, int* n_free_out,
+                           b2d_stream_t stream);
+
+/* Per-head RMS norms of q and k, rotation and paged append for rows of the QKV projection
+ * (qkv_norm_rope GK/kernels.metal:246-304; b2d_rope_kv_append is the one-row form without
+ * norms).  qkv [rows, (Hq + 2 Hkv) * HD] (F32 or F16, row stride ldqkv) is not written.  Per
+ * head: x * rsqrt(mean(x^2) + eps) * gamma with q_gamma / k_gamma [HD] (NULL: no norm), then the
+ * rotation of the pairs (i, i + HD/2) by positions[row] * inv_freq[i] (a zero inv_freq leaves its
+ * pair alone).  v is normalized without a weight if v_norm.  q goes to q_out (F32 or F16, row
+ * stride ldq; qkv itself with ldq = ldqkv is allowed for equal types), k and v rounded to fp16
+ * to slot slots[row] of the pages.  Rows with positions[row] < 0, and rows from *n_rows on (a
+ * device int, e.g. cu_q + batch; NULL: all rows), are skipped; slots outside [0, n_blocks * 16)
+ * (or slots NULL) store nothing.  Two rows with the same slot leave either's values there.
+ * head_dim 64, 128 or 256.  Angles are exact to fp32 for positions below 2^24. */
+B2D_API int b2d_qk_norm_rope_append(const void* qkv, int qkv_dtype, int ldqkv,
+                                    const float* q_gamma, const float* k_gamma, float eps,
+                                    int v_norm, const int* positions, const long long* slots,
+                                    const int* n_rows, const float* inv_freq, void* q_out,
+                                    int q_dtype, int ldq, uint16_t* k_pages, uint16_t* v_pages,
+                                    int n_blocks, int n_heads, int n_kv_heads, int head_dim,
+                                    int rows, b2d_stream_t stream);
+
+/* Attention of the rows cu_q[b] .. cu_q[b + 1] of each sequence over its paged cache (attention
+ * LK/kernels.metal:235-305; b2d_paged_decode_attn is the one-row form).  q [rows, Hq * HD] (F32 or
+ * F16, row stride ldq) is rotated already, and the rows' own k and v are in the cache at places
+ * ctx_lens[b] + i.  Row i sees the places before ctx_lens[b] and, of the step's own rows, those
+ * with its bit set in mask[row][mask_words] (a drafted tree; mask_words <= 8), or with mask NULL
+ * the rows up to itself.  window > 0 further hides every place whose position is <= the row's
+ * position - window: positions are the places themselves, except that with a mask the step's own
+ * rows have positions[row] (required then; b2d_paged_plan's).  A row that sees nothing gives
+ * zeros.  What a hidden place holds (infinities and NaN included) changes nothing.
+ * out [rows, Hq * HD] (F32, F16 or F16X2 with its lo plane at out + rows * ldout).  fp16 q with an
+ * fp16 output multiplies in fp16 with fp32 sums; every other combination carries q and the
+ * weights as hi + lo fp16 pairs.  head_dim 64, 128 or 256; n_heads / n_kv_heads <= 64.
+ * max_q bounds the rows of a sequence and max_ctx every ctx_lens[b] + rows (a sequence beyond
+ * max_ctx, and rows beyond max_q, are left as they were).  Block-table entries outside
+ * [0, n_blocks) are never dereferenced; their places are hidden.  scale <= 0 means
+ * 1/sqrt(head_dim).
+ * Workspace: b2d_paged_tree_attn_workspace_bytes() bytes (may be 0), any contents; it holds
+ * nothing between calls, and calls that may overlap need one each.
+ * b2d_paged_tree_attn_error waits for the device and returns B2D_ERR_TIMEOUT if a bounded wait of
+ * a call on the current device gave up since the last query (its output is incomplete). */
+B2D_API size_t b2d_paged_tree_attn_workspace_bytes(int batch, int rows, int n_heads,
+                                                   int n_kv_heads, int head_dim, int max_q,
+                                                   int max_ctx);
+B2D_API int b2d_paged_tree_attn_error(void);
+B2D_API int b2d_paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages,
+                                const uint16_t* v_pages, const int* block_table, int max_blocks,
+                                int n_blocks, const int* ctx_lens, const int* cu_q,
+                                const uint32_t* mask, int mask_words, const int* positions,
+                                int n_heads, int n_kv_heads, int head_dim, int batch, int rows,
+                                int max_q, int max_ctx, float scale, int window, void* out,
+                                int out_dtype, int ldout, void* workspace, size_t workspace_bytes,
+                                b2d_stream_t stream);
+
+/* Log probabilities of given tokens, entropy and top alternatives of rows of logits (the scoring
+ * side of argmax, LK/kernels.metal:310-345).  logits [rows, V] (F32 or F16, row stride ld, any
+ * alignment).  With lse = log(sum_i exp(x_i)):
+ *   logprobs[row][j] = x[targets[row][j]] - lse   for j < n_targets (-inf for ids outside [0, V))
+ *   entropy[row] = lse - sum_i p_i x_i            (NULL to skip), in nats
+ *   top_ids / top_logprobs[row][j], j < top_k <= 32: the largest logits in falling order, equal
+ *   ones by rising index.
+ * A row of -inf only has log probabilities -inf and entropy 0; a NaN or +inf makes a row's
+ * probabilities and entropy NaN, its ids still follow the order (NaN last).  Rows from *n_rows on
+ * (a device int; NULL: all rows) are skipped. */
+B2D_API int b2d_token_logprobs(const void* logits, int dtype, long long ld, int V, int rows,
+                               const int* n_rows, const int* targets, int n_targets, int top_k,
+                               float* logprobs, float* entropy, int* top_ids,
+                               float* top_logprobs, b2d_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
  * Decode step of a Llama-style model (Engine.encodeDecode LK/main.swift:321-347), ragged
  * batch over a paged cache, optionally tensor-parallel over NCCL.
  * ------------------------------------------------------------------------------------- */

@@ -306,3 +306,174 @@ def paged_decode_attention(
         V = gather_kv(v_pages, block_table[b], n)
         out[b] = attention(qr[b], K, V, scale, window).reshape(-1)
     return out
+
+
+# --------------------------------------------------------------------------------------------
+# Several rows per sequence: drafted tokens and prompt chunks (extension, include/b200dec.h)
+# --------------------------------------------------------------------------------------------
+
+PLAN_OK, PLAN_PAGES, PLAN_TABLE, PLAN_ROWS, PLAN_TREE = 0, 1, 2, 3, 4
+
+
+def tree_bits(parents) -> tuple[np.ndarray, np.ndarray]:
+    """bits[i, j]: node j is node i or an ancestor of it; depth[i].  A parent that is not an earlier
+    node is the root."""
+    n = len(parents)
+    bits, depth = np.eye(n, dtype=bool), np.zeros(n, np.int64)
+    for i, p in enumerate(parents):
+        if 0 <= p < i:
+            bits[i] |= bits[p]
+            depth[i] = depth[p] + 1
+    return bits, depth
+
+
+def pack_bits(bits, words: int) -> np.ndarray:
+    out = np.zeros((bits.shape[0], 32 * words), np.uint8)
+    out[:, : bits.shape[1]] = bits
+    return np.packbits(out, axis=1, bitorder="little").view(np.int32)
+
+
+def paged_plan(ctx, q, table, n_pages, stack, n_free, max_tokens: int, parents=None, words: int = 0) -> dict:
+    """b2d_paged_plan on copies; rows behind the last request come back as -9."""
+    B, mb = table.shape
+    table, stack = table.copy(), stack.copy()
+    top = int(n_free)
+    for b in range(B):
+        if q[b] < 0:
+            for j in range(int(n_pages[b])):
+                if top < len(stack):
+                    stack[top] = table[b, j]
+                top += 1
+    top = min(top, len(stack))
+    cu, status, own, asked, given = [0], [], [], 0, 0
+    slots, positions = np.full(max_tokens, -9, np.int64), np.full(max_tokens, -9, np.int32)
+    mask = np.full((max_tokens, words), -9, np.int32)
+    end = 0
+    for b in range(B):
+        n, have, c = max(int(q[b]), 0), int(n_pages[b]), int(ctx[b])
+        end += n
+        st, want = PLAN_OK, 0
+        if q[b] >= 0:
+            pages = -(-(c + n) // PAGE_TOKENS)
+            if end > max_tokens:
+                st = PLAN_ROWS
+            elif c < 0 or pages > mb:
+                st = PLAN_TABLE
+            elif words and n > 32 * words:
+                st = PLAN_TREE
+            else:
+                want = max(0, pages - have)
+                if want and asked + want > top:
+                    st = PLAN_PAGES
+        for j in range(want if st == PLAN_OK else 0):
+            table[b, have + j] = stack[top - 1 - asked - j]
+        given += want if st == PLAN_OK else 0
+        asked += want
+        own.append(0 if q[b] < 0 else have + (want if st == PLAN_OK else 0))
+        status.append(st)
+        r0, r1 = cu[-1], min(end, max_tokens)
+        cu.append(r1)
+        k = r1 - r0
+        positions[r0:r1] = c + np.arange(k)
+        if words and k:
+            bits, depth = tree_bits(parents[r0:r1])
+            if k <= 32 * words:
+                positions[r0:r1] = c + depth
+                mask[r0:r1] = pack_bits(bits, words)
+            else:
+                mask[r0:r1] = 0
+        for i in range(k):
+            pg = table[b, (c + i) // PAGE_TOKENS] if st == PLAN_OK else -1
+            slots[r0 + i] = pg * PAGE_TOKENS + (c + i) % PAGE_TOKENS if pg >= 0 else -1
+    i32 = lambda a: np.array(a, np.int32)  # noqa: E731
+    return dict(cu_q=i32(cu), slots=slots, positions=positions, mask=mask, status=i32(status), n_pages=i32(own),
+                n_free=i32([top - given]), table=table, stack=stack)
+
+
+def qk_norm_rope(qkv, positions, invf, hq: int, hk: int, hd: int, q_gamma=None, k_gamma=None, eps=1e-6, v_norm=False):
+    """Rows of q, k and v after b2d_qk_norm_rope_append, unrounded (angles exact; GK/kernels.metal:246-304)."""
+    x = f64(qkv).reshape(len(qkv), hq + 2 * hk, hd)
+    q, k, v = x[:, :hq], x[:, hq : hq + hk], x[:, hq + hk :]
+    if q_gamma is not None:
+        q = rmsnorm(q, q_gamma, eps)
+    if k_gamma is not None:
+        k = rmsnorm(k, k_gamma, eps)
+    if v_norm:
+        v = rmsnorm(v, np.ones(hd), eps)
+    a = f64(positions)[:, None, None] * f64(invf)
+    c, s = np.cos(a), np.sin(a)
+
+    def turn(t):
+        lo, hi = t[..., : hd // 2], t[..., hd // 2 :]
+        return np.concatenate([lo * c - hi * s, hi * c + lo * s], -1)
+
+    return turn(q), turn(k), v
+
+
+def tree_attention(q, k_pages, v_pages, table, ctx, cu, hq, hk, hd, bits=None, positions=None, scale=0.0, window=0):
+    """b2d_paged_tree_attn: rows q [R, hq * hd]; bits[r] (truth values over the sequence's own rows) or
+    None for the rows up to itself.  Returns the output and sum_j p_j |v_j| (for error bounds), both
+    [R, hq, hd]; rows outside every sequence are NaN."""
+    R = len(q)
+    out = np.full((R, hq, hd), np.nan)
+    mag = np.zeros((R, hq, hd))
+    scale = scale if scale > 0 else hd**-0.5
+    G = hq // hk
+    for b in range(len(ctx)):
+        r0, T, c = int(cu[b]), int(cu[b + 1] - cu[b]), int(ctx[b])
+        if T <= 0:
+            continue
+        n = c + T
+        ids = np.array([table[b, j // PAGE_TOKENS] for j in range(n)])
+        have = (ids >= 0) & (ids < len(k_pages))
+        at = np.arange(n) % PAGE_TOKENS
+        K = f64(k_pages[np.where(have, ids, 0), :, at])  # [n, hk, hd]
+        V = f64(v_pages[np.where(have, ids, 0), :, at])
+        place = np.arange(n)
+        pos = place.copy()
+        if bits is not None and positions is not None:
+            pos[c:] = positions[r0 : r0 + T]
+        for i in range(T):
+            see = have & ((place < c) | (place - c <= i))
+            if bits is not None:
+                see = have & ((place < c) | np.concatenate([np.zeros(c, bool), bits[r0 + i][:T]]))
+            if window:
+                see &= pos > (positions[r0 + i] if bits is not None else c + i) - window
+            for h in range(hq):
+                if not see.any():
+                    out[r0 + i, h] = 0
+                    continue
+                s = K[see, h // G] @ f64(q[r0 + i, h * hd : (h + 1) * hd]) * scale
+                with np.errstate(invalid="ignore", over="ignore"):
+                    p = np.exp(s - s.max())
+                    p /= p.sum()
+                    out[r0 + i, h] = p @ V[see, h // G]
+                    mag[r0 + i, h] = p @ np.abs(V[see, h // G])
+    return out, mag
+
+
+def token_logprobs(logits, targets=None, k: int = 0):
+    """b2d_token_logprobs: (logprobs [R, n] or None, entropy [R], top ids, top logprobs [R, k])."""
+    x = f64(logits)
+    R, V = x.shape
+    with np.errstate(invalid="ignore", divide="ignore"):
+        m = x.max(1, keepdims=True)
+        z = np.where(x == m, 0.0, x - m) if np.isneginf(m).any() else x - m
+        e = np.exp(z)
+        e = np.where(np.isneginf(x), 0.0, e)
+        s = e.sum(1, keepdims=True)
+        # x - m first: the logarithm would be lost next to a large m
+        lp = np.where(np.isneginf(m), x, (x - m) - np.log(s))
+        ent = -(np.where(e > 0, (e / s) * (z - np.log(s)), 0.0)).sum(1)
+        broken = np.isnan(x).any(1) | np.isposinf(x).any(1)
+        lp[broken], ent[broken] = np.nan, np.nan
+    tl = None
+    if targets is not None:
+        t = np.asarray(targets).reshape(R, -1)
+        ok = (t >= 0) & (t < V)
+        tl = np.where(ok, np.take_along_axis(lp, np.where(ok, t, 0), 1), -np.inf)
+        tl[broken] = np.nan
+    order = np.where(np.isnan(x), -np.inf, x)
+    # NaN behind -inf: a second key
+    ids = np.stack([np.lexsort((np.arange(V), -order[r], np.isnan(x[r]))) for r in range(R)])[:, :k]
+    return tl, ent, ids, np.take_along_axis(lp, ids, 1)
