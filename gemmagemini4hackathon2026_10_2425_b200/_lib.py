@@ -151,13 +151,18 @@ def call(name: str, *args) -> int:
     """Call an entry point; translate a non-zero status into ValueError / RuntimeError."""
     st = getattr(lib(), name)(*args)
     if st != OK:
-        msg = lib().b2d_status_string(st).decode()
-        if st == ERR_CUDA:
-            msg += f" (cudaError {lib().b2d_last_cuda_error()})"
-        if st in (ERR_NULL, ERR_SHAPE, ERR_ALIGN, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_STATE):
-            raise ValueError(f"{name}: {msg} (status {st})")
-        raise B2DError(name, st, msg)
+        raise_status(name, st)
     return st
+
+
+def raise_status(name: str, st: int) -> None:
+    """The exception of a non-zero status."""
+    msg = lib().b2d_status_string(st).decode()
+    if st == ERR_CUDA:
+        msg += f" (cudaError {lib().b2d_last_cuda_error()})"
+    if st in (ERR_NULL, ERR_SHAPE, ERR_ALIGN, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_STATE):
+        raise ValueError(f"{name}: {msg} (status {st})")
+    raise B2DError(name, st, msg)
 
 
 def declared_symbols() -> list[str]:

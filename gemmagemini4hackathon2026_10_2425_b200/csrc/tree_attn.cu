@@ -49,6 +49,7 @@ struct Params {
   const void* q;
   int q_f16;
   long long ldq;
+  const uint16_t* k_pages;
   const uint16_t* v_pages;
   const int* block_table;
   int max_blocks, n_blocks;
@@ -57,7 +58,8 @@ struct Params {
   const uint32_t* mask;
   int words;
   const int* positions;
-  int n_heads, n_kv, rows, max_q, max_ctx;
+  int n_heads, n_kv, batch, rows, max_q, max_ctx;
+  int m_tiles;  // row tiles of the longest sequence
   float scale_log2;  // scale * log2(e)
   int window;
   void* out;
@@ -70,39 +72,33 @@ struct Params {
   float* part_ml;  // [rows][n_heads][max_chunks][2]
 };
 
-// What a CTA of (sequence b, 64-row tile) works on; the same in both kernels.
+
+// What the row tile m0 .. m1 - 1 of sequence b works on; the same in every kernel.
 struct Span {
-  int row0, T, ctx;   // first row, rows, cached places
-  int lo, hi;         // places [lo, hi) that any of the tile's rows may see; lo a multiple of kKeys
-  int pmin, pmax;     // smallest and largest position of the tile's rows
+  int row0, T, ctx;  // first row, rows, cached places
+  int lo, hi;        // places [lo, hi) that any of the tile's rows may see; lo a multiple of `keys`
+  int pmax;          // no row's position is larger
   __device__ int chunks(int chunk) const { return hi > lo ? (hi - lo + chunk - 1) / chunk : 0; }
 };
 
-__device__ __forceinline__ bool span_of(const Params& p, int b, int m0, int m1, int G, Span& s) {
+__device__ __forceinline__ bool span_of(const Params& p, int b, int m0, int m1, int G, int keys, Span& s) {
   s.ctx = p.ctx_lens[b];
   s.row0 = p.cu_q[b];
   s.T = min(min(p.cu_q[b + 1] - s.row0, p.max_q), p.rows - s.row0);
   if (s.row0 < 0 || s.T <= 0 || s.ctx < 0 || s.ctx > p.max_ctx - s.T) return false;
   const int t0 = m0 / G, t1 = min((m1 - 1) / G, s.T - 1);  // the tile's rows
   if (t0 >= s.T) return false;
-  s.pmin = s.ctx + t0;
   s.pmax = s.ctx + t1;
-  if (p.window > 0 && p.mask) {
-    s.pmin = INT_MAX;
-    s.pmax = INT_MIN;
-    for (int t = t0 + (threadIdx.x & 31); t <= t1; t += 32) {
-      const int pos = p.positions[s.row0 + t];
-      s.pmin = min(s.pmin, pos);
-      s.pmax = max(s.pmax, pos);
-    }
-    s.pmin = __reduce_min_sync(0xffffffffu, s.pmin);
-    s.pmax = __reduce_max_sync(0xffffffffu, s.pmax);
-  }
   s.hi = p.mask ? s.ctx + s.T : s.ctx + t1 + 1;
-  // places up to pmin - window are outside every row's window (the step's own rows are kept: their
-  // positions need not rise with their places)
-  s.lo = p.window > 0 ? max(0, min(s.pmin - p.window + 1, s.ctx)) / kKeys * kKeys : 0;
+  // row t's position is at least ctx (a tree) or ctx + t
+  s.lo = p.window > 0 ? max(0, min(s.ctx + (p.mask ? 0 : t0) - p.window + 1, s.ctx)) / keys * keys : 0;
   return true;
+}
+
+// Position of row i of a sequence: given ones are held to ctx .. ctx + i, where a tree's are.
+__device__ __forceinline__ int row_position(const Params& p, const Span& s, int i) {
+  if (!p.mask || p.window <= 0) return s.ctx + i;
+  return min(max(p.positions[s.row0 + i], s.ctx), s.ctx + i);
 }
 
 template <int HD>
@@ -162,6 +158,51 @@ __device__ __forceinline__ void consumers_sync() {
   asm volatile("bar.sync 1, 128;" ::: "memory");
 }
 
+// 8 elements of a q row as fp16, and what fp32 elements have beyond that.
+__device__ __forceinline__ void q_chunk(const Params& p, int row, int head, int hd, int ch, uint4& h, uint4& l) {
+  const long long at = (long long)row * p.ldq + (long long)head * hd + ch * 8;
+  if (p.q_f16) {
+    h = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at);
+  } else {
+    const float4 u = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at);
+    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at + 4);
+    h = make_uint4(pack2(u.x, u.y), pack2(u.z, u.w), pack2(v.x, v.y), pack2(v.z, v.w));
+    l = make_uint4(pack2_rest(u.x, u.y, h.x), pack2_rest(u.z, u.w, h.y), pack2_rest(v.x, v.y, h.z),
+                   pack2_rest(v.z, v.w, h.w));
+  }
+}
+// Any of 8 fp16 values infinite or NaN.
+__device__ __forceinline__ bool nonfinite(uint4 u) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  bool any = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) any |= (w[e] & 0x7c00u) == 0x7c00u || (w[e] & 0x7c000000u) == 0x7c000000u;
+  return any;
+}
+
+// 32 consecutive output elements from i on (16-byte aligned).
+__device__ __forceinline__ void store_row32(const Params& p, long long i, const float* v) {
+  if (!p.out_f16) {
+    float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + i);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+    return;
+  }
+  uint32_t h[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) h[e] = pack2(v[2 * e], v[2 * e + 1]);
+  uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + i);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
+  if (p.out_lo) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) h[e] = pack2_rest(v[2 * e], v[2 * e + 1], h[e]);
+    o = reinterpret_cast<uint4*>(p.out_lo + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
+  }
+}
+
 __device__ __forceinline__ void store_out(const Params& p, long long i, float v) {
   if (p.out_f16)
     store_f16_split(static_cast<uint16_t*>(p.out), p.out_lo, (size_t)i, v);
@@ -169,18 +210,21 @@ __device__ __forceinline__ void store_out(const Params& p, long long i, float v)
     static_cast<float*>(p.out)[i] = v;
 }
 
-// q . k of one row's head and key r of a tile, in fp32.
-template <int HD>
-__device__ __noinline__ float dot_row(const Params& p, int row, int head, const uint8_t* Kt, int r) {
+// q . k of one row's head and a key, in fp32.
+template <int HD, class Key>
+__device__ __forceinline__ float dot_row(const Params& p, int row, int head, Key key) {
   const long long at = (long long)row * p.ldq + (long long)head * HD;
   float a = 0.f;
-  for (int d = 0; d < HD; ++d) {
-    const float k = h2f(*reinterpret_cast<const uint16_t*>(Kt + sw(r, d / 8, kKeys) + (d & 7) * 2));
-    const float q = p.q_f16 ? h2f(static_cast<const uint16_t*>(p.q)[at + d])
-                            : static_cast<const float*>(p.q)[at + d];
-    a = fmaf(q, k, a);
-  }
+  for (int d = 0; d < HD; ++d)
+    a = fmaf(p.q_f16 ? h2f(static_cast<const uint16_t*>(p.q)[at + d]) : static_cast<const float*>(p.q)[at + d],
+             key(d), a);
   return a;
+}
+template <int HD>
+__device__ __noinline__ float dot_tile(const Params& p, int row, int head, const uint8_t* Kt, int r) {
+  return dot_row<HD>(p, row, head, [&](int d) {
+    return h2f(*reinterpret_cast<const uint16_t*>(Kt + sw(r, d / 8, kKeys) + (d & 7) * 2));
+  });
 }
 
 template <int HD, bool X2>
@@ -197,12 +241,12 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
   __shared__ int failed;
 
   const int G = p.n_heads / p.n_kv;
-  const int m_tiles = (p.max_q * G + kRows - 1) / kRows;
+  const int m_tiles = p.m_tiles;
   const int c = blockIdx.x, b = blockIdx.z;
   const int kvh = blockIdx.y / m_tiles, m0 = (blockIdx.y % m_tiles) * kRows;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   Span s;
-  if (!span_of(p, b, m0, m0 + kRows, G, s)) return;
+  if (!span_of(p, b, m0, m0 + kRows, G, kKeys, s)) return;
   const int nact = s.chunks(p.chunk);
   if (c >= max(nact, 1)) return;
   const int lo = s.lo + c * p.chunk, hi = min(lo + p.chunk, s.hi);
@@ -229,18 +273,7 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
     const int r = i / (HD / 8), ch = i % (HD / 8);
     const int m = m0 + r, t = m / G, g = m % G;
     uint4 h = make_uint4(0u, 0u, 0u, 0u), l = h;
-    if (t < s.T) {
-      const long long at = (long long)(s.row0 + t) * p.ldq + (long long)(kvh * G + g) * HD + ch * 8;
-      if (p.q_f16) {
-        h = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at);
-      } else {
-        const float4 u = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at);
-        const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at + 4);
-        h = make_uint4(pack2(u.x, u.y), pack2(u.z, u.w), pack2(v.x, v.y), pack2(v.z, v.w));
-        l = make_uint4(pack2_rest(u.x, u.y, h.x), pack2_rest(u.z, u.w, h.y),
-                       pack2_rest(v.x, v.y, h.z), pack2_rest(v.z, v.w, h.w));
-      }
-    }
+    if (t < s.T) q_chunk(p, s.row0 + t, kvh * G + g, HD, ch, h, l);
     *reinterpret_cast<uint4*>(qs + sw(r, ch, kRows)) = h;
     if (X2) *reinterpret_cast<uint4*>(qs + C::Q_PLANE + sw(r, ch, kRows)) = l;
   }
@@ -286,7 +319,7 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
     int pos[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      pos[e] = (p.window > 0 && p.mask && live[e]) ? p.positions[s.row0 + ts[e]] : s.ctx + ts[e];
+      pos[e] = live[e] ? row_position(p, s, ts[e]) : s.ctx;
     const uint32_t* words[2] = {p.mask + (long long)(s.row0 + (live[0] ? ts[0] : 0)) * p.words,
                                 p.mask + (long long)(s.row0 + (live[1] ? ts[1] : 0)) * p.words};
     float o[ND][4];
@@ -316,16 +349,11 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
           const int r = x / (HD / 8), ch = x % (HD / 8);
           uint4* v = reinterpret_cast<uint4*>(Vt + sw(r, ch, kKeys));
           const bool out = j0 + r >= s.hi || blk[i * (kKeys / 16) + r / 16] < 0;
-          bool nonfinite = false;
           if (!out) {
-            const uint4 u = *v;
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              nonfinite |= (w[e] & 0x7c00u) == 0x7c00u || (w[e] & 0x7c000000u) == 0x7c000000u;
-            if (nonfinite) atomicOr(&bad_keys, 1ull << r);
+            if (nonfinite(*v)) atomicOr(&bad_keys, 1ull << r);
+          } else {
+            *v = make_uint4(0u, 0u, 0u, 0u);
           }
-          if (out) *v = make_uint4(0u, 0u, 0u, 0u);
         }
         consumers_sync();
         bad = *reinterpret_cast<volatile unsigned long long*>(&bad_keys);
@@ -374,7 +402,7 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (sc[n][e] != sc[n][e] && live[e >> 1])
-                sc[n][e] = dot_row<HD>(p, s.row0 + ts[e >> 1], kvh * G + (mr0 + 8 * (e >> 1)) % G, Kt,
+                sc[n][e] = dot_tile<HD>(p, s.row0 + ts[e >> 1], kvh * G + (mr0 + 8 * (e >> 1)) % G, Kt,
                                        n * 8 + 2 * t4 + (e & 1));
         }
       }
@@ -392,7 +420,7 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
                            : own <= ts[h];
             }
             if (see && p.window > 0) {
-              const int kp = (p.mask && j >= s.ctx) ? p.positions[s.row0 + j - s.ctx] : j;
+              const int kp = j >= s.ctx ? row_position(p, s, j - s.ctx) : j;
               see = kp > pos[h] - p.window;
             }
             if (!see) sc[n][e] = -INFINITY;
@@ -521,11 +549,11 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
 template <int HD>
 __global__ void __launch_bounds__(256) tree_join_kernel(const Params p) {
   const int G = p.n_heads / p.n_kv;
-  const int m_tiles = (p.max_q * G + kRows - 1) / kRows;
+  const int m_tiles = p.m_tiles;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, kvh = blockIdx.y / m_tiles, m0 = (blockIdx.y % m_tiles) * kRows;
   Span s;
-  if (!span_of(p, b, m0, m0 + kRows, G, s)) return;
+  if (!span_of(p, b, m0, m0 + kRows, G, kKeys, s)) return;
   const int nact = s.chunks(p.chunk);
   const int m = m0 + blockIdx.x * 8 + warp, t = m / G, head = kvh * G + m % G;
   if (nact <= 1 || t >= s.T) return;
@@ -578,6 +606,14 @@ static Plan plan_of(int batch, int rows, int n_heads, int n_kv, int head_dim, in
   return pl;
 }
 
+}  // namespace tree
+}  // namespace b2d
+
+#include "tree_attn_t5.cuh"
+
+namespace b2d {
+namespace tree {
+
 template <int HD, bool X2>
 static int launch(const Params& p, int m_tiles, int batch, cudaStream_t stream) {
   auto kern = paged_tree_attn_kernel<HD, X2>;
@@ -605,10 +641,18 @@ static bool shape_ok(int batch, int rows, int n_heads, int n_kv, int max_q, int 
 
 }  // namespace tree
 
+// The larger of the two operand forms' needs: the query does not know the types.
 size_t paged_tree_attn_workspace_bytes(int batch, int rows, int n_heads, int n_kv_heads, int head_dim,
                                        int max_q, int max_ctx) {
   if (!tree::shape_ok(batch, rows, n_heads, n_kv_heads, max_q, max_ctx) || head_dim <= 0) return 0;
-  return tree::plan_of(batch, rows, n_heads, n_kv_heads, head_dim, max_q, max_ctx).bytes;
+  size_t need = 0;
+  for (const bool x2 : {false, true}) {
+    const tree::t5::Shape h = tree::t5::shape_of(batch, n_heads, n_kv_heads, head_dim, max_q, max_ctx, x2);
+    need = std::max(need, tree::t5::serves(head_dim, batch, h.max_steps)
+                              ? h.bytes
+                              : tree::plan_of(batch, rows, n_heads, n_kv_heads, head_dim, max_q, max_ctx).bytes);
+  }
+  return need;
 }
 
 int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages,
@@ -631,8 +675,9 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) ||
       ldq % (q_dtype == B2D_F16 ? 8 : 4) || ldout % (out_dtype == B2D_F32 ? 4 : 8))
     return B2D_ERR_ALIGN;
-  const tree::Plan pl = tree::plan_of(batch, rows, n_heads, n_kv_heads, head_dim, max_q, max_ctx);
-  if (pl.bytes && (!workspace || workspace_bytes < pl.bytes)) return B2D_ERR_WORKSPACE;
+  const size_t need =
+      paged_tree_attn_workspace_bytes(batch, rows, n_heads, n_kv_heads, head_dim, max_q, max_ctx);
+  if (need && (!workspace || workspace_bytes < need)) return B2D_ERR_WORKSPACE;
   if (!aligned16(workspace)) return B2D_ERR_ALIGN;
   tree::Params p = {};
   const uint64_t prows = (uint64_t)n_blocks * n_kv_heads * 16;
@@ -642,6 +687,7 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
   p.q = q;
   p.q_f16 = q_dtype == B2D_F16;
   p.ldq = ldq;
+  p.k_pages = k_pages;
   p.v_pages = v_pages;
   p.block_table = block_table;
   p.max_blocks = max_blocks;
@@ -653,6 +699,7 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
   p.positions = positions;
   p.n_heads = n_heads;
   p.n_kv = n_kv_heads;
+  p.batch = batch;
   p.rows = rows;
   p.max_q = max_q;
   p.max_ctx = max_ctx;
@@ -662,11 +709,25 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
   p.out_f16 = out_dtype != B2D_F32;
   p.out_lo = out_dtype == B2D_F16X2 ? static_cast<uint16_t*>(out) + (size_t)rows * ldout : nullptr;
   p.ldout = ldout;
+  p.part_o = static_cast<float*>(workspace);
+  const bool x2 = q_dtype == B2D_F32 || out_dtype != B2D_F16;
+  const tree::t5::Shape h = tree::t5::shape_of(batch, n_heads, n_kv_heads, head_dim, max_q, max_ctx, x2);
+  if (tree::t5::serves(head_dim, batch, h.max_steps)) {
+    p.m_tiles = h.m_tiles;
+    p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + h.off_ml);
+    if (head_dim == 64)
+      return h.mt2 ? tree::t5::launch<64, true, false>(p, h, stream)
+                   : (x2 ? tree::t5::launch<64, false, true>(p, h, stream)
+                         : tree::t5::launch<64, false, false>(p, h, stream));
+    return h.mt2 ? tree::t5::launch<128, true, false>(p, h, stream)
+                 : (x2 ? tree::t5::launch<128, false, true>(p, h, stream)
+                       : tree::t5::launch<128, false, false>(p, h, stream));
+  }
+  const tree::Plan pl = tree::plan_of(batch, rows, n_heads, n_kv_heads, head_dim, max_q, max_ctx);
+  p.m_tiles = pl.m_tiles;
   p.chunk = pl.chunk;
   p.max_chunks = pl.max_chunks;
-  p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.off_ml);
-  const bool x2 = q_dtype == B2D_F32 || out_dtype != B2D_F16;
   switch (head_dim) {
     case 64: return x2 ? tree::launch<64, true>(p, pl.m_tiles, batch, stream)
                        : tree::launch<64, false>(p, pl.m_tiles, batch, stream);

@@ -18,12 +18,13 @@ current stream of their tensors' device, keep nothing between calls and use no s
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib
-from ._lib import call
+from ._lib import call, raise_status
 
 _DT = {torch.float32: _lib.F32, torch.float16: _lib.F16}
 EPILOGUES = {
@@ -631,22 +632,29 @@ def add_rmsnorm_f16(x: torch.Tensor, gamma: torch.Tensor, eps: float, p: torch.T
 # -- several rows per sequence: drafted tokens and prompt chunks ---------------------------------
 
 
-def _check(name: str, t: torch.Tensor | None, dtypes, dev: torch.device, shape=None, rows: bool = False) -> None:
-    """t (None passes) is on dev, of one of dtypes and of `shape` (None entries are free), contiguous
-    (with rows: only each row is, at any row stride)."""
-    if t is None:
+def _check(name: str, t: torch.Tensor | None, dtypes, d: int, shape, rows: bool = False) -> None:
+    """t (None passes) is on CUDA device d, of one of dtypes and of `shape`, contiguous (with rows: only
+    each row is, at any row stride)."""
+    if t is None or t.dtype in dtypes and t.get_device() == d and t.shape == shape and t.is_contiguous():
         return
-    if not t.is_cuda or t.device != dev:
-        raise ValueError(f"{name} must be a CUDA tensor on {dev} (no CPU path exists)")
+    if not t.is_cuda or t.get_device() != d:
+        raise ValueError(f"{name} must be a CUDA tensor on the device of the first one (no CPU path exists)")
     if t.dtype not in dtypes:
-        raise ValueError(f"{name} has dtype {t.dtype}, expected one of {[str(d) for d in dtypes]}")
-    if shape is not None and (t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape))):
+        raise ValueError(f"{name} has dtype {t.dtype}, expected one of {[str(x) for x in dtypes]}")
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {list(t.shape)}, expected {list(shape)}")
-    if rows:
-        if t.stride(-1) != 1 and t.shape[-1] > 1 or t.dim() == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-            raise ValueError(f"{name} needs contiguous rows that do not overlap")
-    elif not t.is_contiguous():
+    if not rows:
         raise ValueError(f"{name} must be contiguous")
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name} needs contiguous rows that do not overlap")
+
+
+def _on_gpu(t: torch.Tensor) -> int:
+    """The CUDA device of a wrapper's first tensor."""
+    d = t.get_device()
+    if d < 0:
+        raise ValueError("all tensors must be CUDA tensors (no CPU path exists)")
+    return d
 
 
 def _ld(t: torch.Tensor) -> int:
@@ -654,14 +662,20 @@ def _ld(t: torch.Tensor) -> int:
     return max(t.stride(0), t.shape[1])
 
 
-def _call_on(dev: torch.device, name: str, *args) -> None:
-    """call() with the current stream of dev as the last argument, on dev."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if dev.index == torch.cuda.current_device():
-        call(name, *args, stream)
+@functools.cache
+def _entry(name: str):
+    return getattr(_lib.lib(), name)
+
+
+def _call_on(d: int, name: str, *args) -> None:
+    """The entry point with the current stream of CUDA device d as its last argument, on that device."""
+    if d == torch.cuda.current_device():
+        st = _entry(name)(*args, torch.cuda.current_stream(d).cuda_stream)
     else:
-        with torch.cuda.device(dev):
-            call(name, *args, stream)
+        with torch.cuda.device(d):
+            st = _entry(name)(*args, torch.cuda.current_stream(d).cuda_stream)
+    if st != _lib.OK:
+        raise_status(name, st)
 
 
 _I32, _I64, _F32, _F16 = (torch.int32,), (torch.int64,), (torch.float32,), (torch.float16,)
@@ -705,15 +719,14 @@ def paged_plan(
     place, n_pages and n_free if `out` holds them.  See include/b200dec.h b2d_paged_plan.  ctx_lens,
     q_lens, n_pages int32 [B]; block_table int32 [B, max_blocks]; free_pages int32 [capacity]; n_free
     int32 [1]; parents int32 [max_tokens] with mask_words (<= 8) words of 32 nodes per row."""
-    dev = ctx_lens.device
-    B = ctx_lens.numel()
-    _check("ctx_lens", ctx_lens, _I32, dev, (B,))
-    _check("q_lens", q_lens, _I32, dev, (B,))
-    _check("block_table", block_table, _I32, dev, (B, None))
-    _check("n_pages", n_pages, _I32, dev, (B,))
-    _check("free_pages", free_pages, _I32, dev, (None,))
-    _check("n_free", n_free, _I32, dev, (1,))
-    _check("parents", parents, _I32, dev, (max_tokens,))
+    dev, d, B = ctx_lens.device, _on_gpu(ctx_lens), ctx_lens.numel()
+    _check("ctx_lens", ctx_lens, _I32, d, (B,))
+    _check("q_lens", q_lens, _I32, d, (B,))
+    _check("block_table", block_table, _I32, d, (B, *block_table.shape[1:2]))
+    _check("n_pages", n_pages, _I32, d, (B,))
+    _check("free_pages", free_pages, _I32, d, (free_pages.numel(),))
+    _check("n_free", n_free, _I32, d, (1,))
+    _check("parents", parents, _I32, d, (max_tokens,))
     if (parents is None) != (mask_words == 0):
         raise ValueError("parents and mask_words go together")
     if out is None:
@@ -728,18 +741,18 @@ def paged_plan(
             torch.empty(1, **i32),
         )
     else:
-        _check("out.cu_q", out.cu_q, _I32, dev, (B + 1,))
-        _check("out.slots", out.slots, _I64, dev, (max_tokens,))
-        _check("out.positions", out.positions, _I32, dev, (max_tokens,))
-        _check("out.status", out.status, _I32, dev, (B,))
-        _check("out.n_pages", out.n_pages, _I32, dev, (B,))
-        _check("out.n_free", out.n_free, _I32, dev, (1,))
+        _check("out.cu_q", out.cu_q, _I32, d, (B + 1,))
+        _check("out.slots", out.slots, _I64, d, (max_tokens,))
+        _check("out.positions", out.positions, _I32, d, (max_tokens,))
+        _check("out.status", out.status, _I32, d, (B,))
+        _check("out.n_pages", out.n_pages, _I32, d, (B,))
+        _check("out.n_free", out.n_free, _I32, d, (1,))
         if mask_words:
             if out.mask is None:
                 raise ValueError("out.mask is missing")
-            _check("out.mask", out.mask, _I32, dev, (max_tokens, mask_words))
+            _check("out.mask", out.mask, _I32, d, (max_tokens, mask_words))
     _call_on(
-        dev,
+        d,
         "b2d_paged_plan",
         ctx_lens.data_ptr(),
         q_lens.data_ptr(),
@@ -764,9 +777,9 @@ def paged_plan(
     return out
 
 
-def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, n_kv_heads: int, head_dim: int, dev: torch.device) -> None:
-    _check("k_pages", k_pages, _F16, dev, (None, n_kv_heads, 16, head_dim))
-    _check("v_pages", v_pages, _F16, dev, tuple(k_pages.shape))
+def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, n_kv_heads: int, head_dim: int, d: int) -> None:
+    _check("k_pages", k_pages, _F16, d, (*k_pages.shape[:1], n_kv_heads, 16, head_dim))
+    _check("v_pages", v_pages, _F16, d, k_pages.shape)
 
 
 def qk_norm_rope_append(
@@ -792,22 +805,22 @@ def qk_norm_rope_append(
     v to their slots, for rows of qkv [R, (Hq + 2 Hkv) * HD]; returns the rotated q [R, Hq * HD].
     See include/b200dec.h b2d_qk_norm_rope_append.  positions int32 [R], slots int64 [R] and n_rows
     (int32 [1], optional: rows in use) as paged_plan returns them."""
-    dev, R, nq = qkv.device, qkv.shape[0], n_heads * head_dim
-    _check("qkv", qkv, _FLOATS, dev, (R, (n_heads + 2 * n_kv_heads) * head_dim), rows=True)
+    dev, d, R, nq = qkv.device, _on_gpu(qkv), qkv.shape[0], n_heads * head_dim
+    _check("qkv", qkv, _FLOATS, d, (R, (n_heads + 2 * n_kv_heads) * head_dim), rows=True)
     if q_out is None:
         q_out = torch.empty(R, nq, dtype=out_dtype, device=dev)
-    _check("q_out", q_out, _FLOATS, dev, (R, nq), rows=True)
-    _check("positions", positions, _I32, dev, (R,))
-    _check("slots", slots, _I64, dev, (R,))
-    _check("inv_freq_dev", inv_freq_dev, _F32, dev, (head_dim // 2,))
-    _check("q_gamma", q_gamma, _F32, dev, (head_dim,))
-    _check("k_gamma", k_gamma, _F32, dev, (head_dim,))
-    _check("n_rows", n_rows, _I32, dev, (1,))
-    _check_pages(k_pages, v_pages, n_kv_heads, head_dim, dev)
+    _check("q_out", q_out, _FLOATS, d, (R, nq), rows=True)
+    _check("positions", positions, _I32, d, (R,))
+    _check("slots", slots, _I64, d, (R,))
+    _check("inv_freq_dev", inv_freq_dev, _F32, d, (head_dim // 2,))
+    _check("q_gamma", q_gamma, _F32, d, (head_dim,))
+    _check("k_gamma", k_gamma, _F32, d, (head_dim,))
+    _check("n_rows", n_rows, _I32, d, (1,))
+    _check_pages(k_pages, v_pages, n_kv_heads, head_dim, d)
     if R == 0:
         return q_out
     _call_on(
-        dev,
+        d,
         "b2d_qk_norm_rope_append",
         qkv.data_ptr(),
         _DT[qkv.dtype],
@@ -866,21 +879,21 @@ def paged_tree_attn(
     HD] is rotated, the rows' k and v are in the cache.  See include/b200dec.h b2d_paged_tree_attn;
     `out` may be fp16 [2, R, Hq * HD]: the output as B2D_F16X2 hi + lo planes.  The workspace (any
     contents) is allocated from torch's caching allocator unless given."""
-    dev, R, nq, B = q.device, q.shape[0], n_heads * head_dim, ctx_lens.numel()
-    _check("q", q, _FLOATS, dev, (R, nq), rows=True)
+    dev, d, R, nq, B = q.device, _on_gpu(q), q.shape[0], n_heads * head_dim, ctx_lens.numel()
+    _check("q", q, _FLOATS, d, (R, nq), rows=True)
     if out is None:
         out = torch.empty(R, nq, dtype=out_dtype, device=dev)
     x2 = _is_x2(out)
     if x2:
-        _check("out", out, _F16, dev, (2, R, nq))
+        _check("out", out, _F16, d, (2, R, nq))
     else:
-        _check("out", out, _FLOATS, dev, (R, nq), rows=True)
-    _check_pages(k_pages, v_pages, n_kv_heads, head_dim, dev)
-    _check("ctx_lens", ctx_lens, _I32, dev, (B,))
-    _check("block_table", block_table, _I32, dev, (B, None))
-    _check("cu_q", cu_q, _I32, dev, (B + 1,))
-    _check("mask", mask, _I32, dev, (R, None))
-    _check("positions", positions, _I32, dev, (R,))
+        _check("out", out, _FLOATS, d, (R, nq), rows=True)
+    _check_pages(k_pages, v_pages, n_kv_heads, head_dim, d)
+    _check("ctx_lens", ctx_lens, _I32, d, (B,))
+    _check("block_table", block_table, _I32, d, (B, *block_table.shape[1:2]))
+    _check("cu_q", cu_q, _I32, d, (B + 1,))
+    _check("mask", mask, _I32, d, (R, *(() if mask is None else mask.shape[1:2])))
+    _check("positions", positions, _I32, d, (R,))
     if R == 0:
         return out
     nbytes = tree_attn_workspace_bytes(B, R, n_heads, n_kv_heads, head_dim, max_q, max_ctx)
@@ -890,7 +903,7 @@ def paged_tree_attn(
     else:
         _check("workspace", workspace, (torch.uint8,), dev, (None,))
     _call_on(
-        dev,
+        d,
         "b2d_paged_tree_attn",
         q.data_ptr(),
         _DT[q.dtype],
@@ -950,15 +963,15 @@ def token_logprobs(
     rows of logits [R, V] (fp32 or fp16, any row stride), each row's entropy, and its top_k <= 32 most
     likely tokens.  See include/b200dec.h b2d_token_logprobs.  Rows from n_rows (int32 [1], on the
     device) on are skipped: pass `out` to keep what it held there."""
-    dev = logits.device
+    dev, d = logits.device, _on_gpu(logits)
     if logits.dim() != 2:
         raise ValueError("logits must be [rows, V]")
     R, V = logits.shape
-    _check("logits", logits, _FLOATS, dev, rows=True)
+    _check("logits", logits, _FLOATS, d, logits.shape, rows=True)
     if targets is not None and (targets.dim() not in (1, 2) or targets.shape[0] != R):
         raise ValueError(f"targets must be int32 [{R}] or [{R}, n]")
-    _check("targets", targets, _I32, dev)
-    _check("n_rows", n_rows, _I32, dev, (1,))
+    _check("targets", targets, _I32, d, None if targets is None else targets.shape)
+    _check("n_rows", n_rows, _I32, d, (1,))
     f32 = dict(dtype=torch.float32, device=dev)
     if out is None:
         out = TokenLogprobs(
@@ -971,15 +984,15 @@ def token_logprobs(
         if (targets is not None and out.logprobs is None) or (top_k > 0 and (out.top_ids is None or out.top_logprobs is None)):
             raise ValueError("out lacks a field that was asked for")
         if targets is not None:
-            _check("out.logprobs", out.logprobs, _F32, dev, tuple(targets.shape))
-        _check("out.entropy", out.entropy, _F32, dev, (R,))
+            _check("out.logprobs", out.logprobs, _F32, d, tuple(targets.shape))
+        _check("out.entropy", out.entropy, _F32, d, (R,))
         if top_k > 0:
-            _check("out.top_ids", out.top_ids, _I32, dev, (R, top_k))
-            _check("out.top_logprobs", out.top_logprobs, _F32, dev, (R, top_k))
+            _check("out.top_ids", out.top_ids, _I32, d, (R, top_k))
+            _check("out.top_logprobs", out.top_logprobs, _F32, d, (R, top_k))
     if R == 0:
         return out
     _call_on(
-        dev,
+        d,
         "b2d_token_logprobs",
         logits.data_ptr(),
         _DT[logits.dtype],

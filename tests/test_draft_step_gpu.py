@@ -358,6 +358,15 @@ def test_attn_long_context_many_chunks(hd, T, tree):
     check_attn(c, torch.float32)
 
 
+@pytest.mark.parametrize("hq,hk,hd,q", [(8, 8, 64, 9), (16, 4, 64, 70), (8, 4, 128, 7), (8, 4, 128, 90), (4, 2, 256, 5)])
+def test_attn_many_sequences(hq, hk, hd, q):
+    """More (sequence, KV head) pairs than SMs, of 1 to several key tiles: a CTA works on several of them."""
+    r = np.random.default_rng(q)
+    c = attn_case(q, r.integers(0, 700, 40), r.integers(0, q + 1, 40), hq, hk, hd, q % 2 == 1)
+    check_attn(c, torch.float16)
+    check_attn(c, torch.float32)
+
+
 def test_attn_widest_tree():
     check_attn(attn_case(8, [37], [256], 4, 2, 64, True), torch.float16)
 
