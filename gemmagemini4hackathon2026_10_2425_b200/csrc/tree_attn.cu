@@ -32,6 +32,7 @@
 namespace b2d {
 
 int make_tmap_f16(CUtensorMap* m, const void* base, uint64_t rows, int cols, int ld, int box_rows);
+int make_tmap_f16_blocks(CUtensorMap* m, const void* base, uint64_t rows, int cols, int box_rows);
 
 namespace tree {
 
@@ -45,7 +46,9 @@ constexpr int kMaxWords = 8;
 __device__ int g_error;  // a bounded wait gave up (b2d_paged_tree_attn_error)
 
 struct Params {
-  CUtensorMap tmK, tmV;  // page pools as [n_blocks * Hkv * 16, HD] fp16, box {64, 16}
+  // page pools as [n_blocks * Hkv * 16, HD] fp16: boxes of 64 columns x 16 rows (tcgen05 kernel's V:
+  // 16 rows x all 64-column blocks)
+  CUtensorMap tmK, tmV;
   const void* q;
   int q_f16;
   long long ldq;
@@ -648,7 +651,7 @@ size_t paged_tree_attn_workspace_bytes(int batch, int rows, int n_heads, int n_k
   size_t need = 0;
   for (const bool x2 : {false, true}) {
     const tree::t5::Shape h = tree::t5::shape_of(batch, n_heads, n_kv_heads, head_dim, max_q, max_ctx, x2);
-    need = std::max(need, tree::t5::serves(head_dim, batch, h.max_steps)
+    need = std::max(need, tree::t5::serves(head_dim, h.max_steps)
                               ? h.bytes
                               : tree::plan_of(batch, rows, n_heads, n_kv_heads, head_dim, max_q, max_ctx).bytes);
   }
@@ -683,7 +686,6 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
   const uint64_t prows = (uint64_t)n_blocks * n_kv_heads * 16;
   if (prows > 0x7fffffffull) return B2D_ERR_SHAPE;
   B2D_TRY(make_tmap_f16(&p.tmK, k_pages, prows, head_dim, head_dim, 16));
-  B2D_TRY(make_tmap_f16(&p.tmV, v_pages, prows, head_dim, head_dim, 16));
   p.q = q;
   p.q_f16 = q_dtype == B2D_F16;
   p.ldq = ldq;
@@ -712,7 +714,8 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
   p.part_o = static_cast<float*>(workspace);
   const bool x2 = q_dtype == B2D_F32 || out_dtype != B2D_F16;
   const tree::t5::Shape h = tree::t5::shape_of(batch, n_heads, n_kv_heads, head_dim, max_q, max_ctx, x2);
-  if (tree::t5::serves(head_dim, batch, h.max_steps)) {
+  if (tree::t5::serves(head_dim, h.max_steps)) {
+    B2D_TRY(make_tmap_f16_blocks(&p.tmV, v_pages, prows, head_dim, 16));
     p.m_tiles = h.m_tiles;
     p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + h.off_ml);
     if (head_dim == 64)
@@ -724,6 +727,7 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
                        : tree::t5::launch<128, false, false>(p, h, stream));
   }
   const tree::Plan pl = tree::plan_of(batch, rows, n_heads, n_kv_heads, head_dim, max_q, max_ctx);
+  B2D_TRY(make_tmap_f16(&p.tmV, v_pages, prows, head_dim, head_dim, 16));
   p.m_tiles = pl.m_tiles;
   p.chunk = pl.chunk;
   p.max_chunks = pl.max_chunks;

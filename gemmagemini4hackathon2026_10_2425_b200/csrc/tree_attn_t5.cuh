@@ -16,8 +16,8 @@
 //   MT2: the warpgroups hold different row tiles (256 rows a unit) and share each K/V tile;
 //   key split: they hold the same 128 rows and take alternate key tiles; their two states meet
 //   through TMEM at the end of the unit.
-// Roles: warps 0-7 softmax (warp w reads TMEM lanes 32 (w % 4) ..), warp 8 TMA, warps 9 and 10
-// issue the MMAs of one warpgroup each.
+// Roles: warps 0-7 softmax (warp w reads TMEM lanes 32 (w % 4) ..), warps 8 and 10 load K and V
+// (TMA), warp 9 issues the MMAs.
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the last time (its
 // weights are then up to 256 and still exact to 2^-11 in fp16), which after the first tiles of a
@@ -33,11 +33,11 @@ namespace t5 {
 
 constexpr int kKeys = 128;
 constexpr int kSoftmax = 256;               // threads of the two warpgroups
-constexpr int kThreads = kSoftmax + 128;    // + TMA warp, two MMA warps, one idle
+constexpr int kThreads = kSoftmax + 128;    // + K, V and MMA warps, one idle
 // Registers: a softmax thread holds a row of 128 scores.  384 threads launch with 168 each
-// (64512); the split 256 * 216 + 128 * 72 uses the same number.
-constexpr int kRegsSoftmax = 216, kRegsOther = 72;
-constexpr int kMaxBatch = 1024;             // prefix sums in shared memory
+// (64512); the split 256 * 224 + 128 * 56 uses the same number.
+constexpr int kRegsSoftmax = 224, kRegsOther = 56;
+constexpr int kGroups = 320;                // prefix sums kept, one per `stride` sequences
 constexpr float kSlack = 8.f;               // log2 of the growth that O is rescaled for
 
 template <int HD, bool MT2, bool X2>
@@ -46,22 +46,13 @@ struct Cfg {
   static constexpr int TILE = kKeys * HD * 2;
   static constexpr int ROWS = MT2 ? 256 : 128;     // rows of a unit
   static constexpr int PLANES = MT2 || X2 ? 2 : 1;  // 128-row fp16 planes of Q
-  static constexpr int SK = HD == 64 ? 4 : (PLANES == 2 ? 2 : 3);
-  static constexpr int SV = HD == 64 ? 4 : 2;
+  // K and V stages.  A V tile waits for the weights, a K tile only for its turn: the room left over
+  // goes to V (HD 128: 2 + 2 stages made the MMAs wait for V 1400 cycles a tile).
+  static constexpr int SK = HD == 64 ? 4 : 2;
+  static constexpr int SV = HD == 64 ? 4 : (X2 ? 2 : 3);
   static constexpr int OFF_K = PLANES * TILE;  // a Q plane is as large as a tile
   static constexpr int OFF_V = OFF_K + SK * TILE;
   static constexpr int OFF_MISC = OFF_V + SV * TILE;
-};
-
-struct Misc {
-  float2 ml[2][128];            // key split: the warpgroups' (reference, sum) per row
-  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
-  uint64_t s_full[2], p_full[2], pv_done[2], q_full[2];
-  unsigned bad[2][4];           // non-finite V rows of the tile at hand
-  unsigned miss[4];             // pages of a V stage's tile that do not exist
-  uint32_t tmem;
-  int failed;
-  int prefix[kMaxBatch + 1];    // first step of each sequence
 };
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
@@ -74,6 +65,42 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
                ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
                : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  return r;
+}
+// Two fp32 operations per instruction.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {  // zeros if not
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -83,32 +110,50 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
 }
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* tm, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+      : "memory");
+}
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
 // 128-byte swizzled operands.  K-major (Q, K): 8-row groups 1024 bytes apart.  MN-major (V, whose
 // rows are the reduction): 8-row groups 1024 bytes apart, 64-column blocks `block` bytes apart.
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-  return (uint64_t)((addr & 0x3FFFF) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t block) {
-  return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(block >> 4) << 16) | (64ull << 32) | (1ull << 46) |
-         (2ull << 61);
+// A descriptor's high word is a constant and its low word holds the address (in 16-byte units,
+// below 2^14, so that adding to it stays in the field) and the block stride: the MMAs of one
+// product differ by an addition of a constant.
+constexpr uint32_t kDescHigh = 64u | (1u << 14) | (2u << 29);  // group stride 1024, version, 128-byte swizzle
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr, uint32_t block) { return (addr >> 4) | ((block >> 4) << 16); }
+// Byte offset of 16-byte chunk ch of row r in a V tile: pages of HD/64 blocks of 16 swizzled rows.
+template <int HD>
+__device__ __forceinline__ uint32_t v_at(int r, int ch) {
+  return (uint32_t)((r >> 4) * (HD * 32) + (ch >> 3) * 2048 + (r & 15) * 128 + (((ch & 7) ^ (r & 7)) << 4));
 }
 // kind::f16, D fp32, A and B fp16, M = 128; bit 16: B is MN-major.
 constexpr uint32_t idesc(int n, bool b_mn) {
   return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, bool acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"((uint32_t)acc));
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 x, {%1, %5};\n\t"
+      "mov.b64 y, {%2, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"((uint32_t)acc), "r"(kDescHigh));
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id) {  // accumulates
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id) {  // accumulates
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(id));
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, 1, 0;\n\tmov.b64 y, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"(kDescHigh));
+}
+// One lane of the warp (the same each time), in code that all of it runs: the operands stay in
+// uniform registers, which a branch on the lane number would load anew for every MMA.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
 // The part of one unit that a CTA works on.
@@ -127,42 +172,53 @@ __device__ __forceinline__ int unit_steps(const Params& p, int b, int mt, int G,
   return max(1, (s.hi - s.lo + kKeys * PER - 1) / (kKeys * PER));
 }
 
-// Prefix sums of the sequences' steps into prefix[0 .. batch]; all threads of the CTA.
+// Steps of sequence b.
 template <int ROWS, int PER>
-__device__ void steps_prefix(const Params& p, int G, int* prefix, int threads) {
-  __shared__ int carry, wsum[32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid == 0) carry = 0;
+__device__ int sequence_steps(const Params& p, int b, int G) {
+  int n = 0;
+  Span s;
+  for (int mt = 0; mt < p.m_tiles; ++mt) {
+    const int u = unit_steps<ROWS, PER>(p, b, mt, G, s);
+    if (u == 0) break;
+    n += u;
+  }
+  return n * p.n_kv;
+}
+
+// prefix[j] = steps of the sequences before j * stride; all threads of the CTA.
+struct Scan {
+  int carry, wsum[32];
+};
+__device__ __forceinline__ int groups_of(int batch, int stride) { return (batch + stride - 1) / stride; }
+template <int ROWS, int PER>
+__device__ void steps_prefix(const Params& p, int G, int stride, int* prefix, Scan& sc) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
+  const int groups = groups_of(p.batch, stride);
+  if (tid == 0) {
+    sc.carry = 0;
+    prefix[0] = 0;
+  }
   __syncthreads();
-  for (int b0 = 0; b0 < p.batch; b0 += threads) {
-    const int b = b0 + tid;
+  for (int j0 = 0; j0 < groups; j0 += threads) {
+    const int j = j0 + tid;
     int n = 0;
-    if (b < p.batch) {
-      Span s;
-      for (int mt = 0; mt < p.m_tiles; ++mt) {
-        const int u = unit_steps<ROWS, PER>(p, b, mt, G, s);
-        if (u == 0) break;
-        n += u;
-      }
-      n *= p.n_kv;
-    }
+    if (j < groups)
+      for (int b = j * stride; b < min((j + 1) * stride, p.batch); ++b) n += sequence_steps<ROWS, PER>(p, b, G);
     int x = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
-    if (lane == 31) wsum[warp] = x;
+    if (lane == 31) sc.wsum[warp] = x;
     __syncthreads();
-    int base = carry;
-    for (int w = 0; w < warp; ++w) base += wsum[w];
-    if (b < p.batch) prefix[b + 1] = base + x;
+    int base = sc.carry;
+    for (int w = 0; w < warp; ++w) base += sc.wsum[w];
+    if (j < groups) prefix[j + 1] = base + x;
     __syncthreads();
-    if (tid == threads - 1) carry = base + x;
+    if (tid == threads - 1) sc.carry = base + x;
     __syncthreads();
   }
-  if (tid == 0) prefix[0] = 0;
-  __syncthreads();
 }
 
 // CTA cta's part of the line of W steps.
@@ -171,39 +227,70 @@ __device__ __forceinline__ int part_begin(int W, int cta, int ctas) { return (in
 // Walks the pieces of steps [x, end) of the line.
 template <int ROWS, int PER>
 struct Walk {
-  int x, end, b;
+  int x, end, b, seq0, seq_end;  // sequence b holds steps [seq0, seq_end)
   bool first;
-  __device__ bool next(const Params& p, const int* prefix, int G, int cta, Piece& pc) {
+  __device__ void begin(int W) {
+    x = part_begin(W, blockIdx.x, gridDim.x);
+    end = part_begin(W, blockIdx.x + 1, gridDim.x);
+    first = true;
+  }
+  __device__ bool next(const Params& p, const int* prefix, int stride, int G, Piece& pc) {
     if (x >= end) return false;
-    if (first) {  // the sequence that holds step x
-      int lo = 0, hi = p.batch;
+    if (first) {  // the group of sequences that holds step x, and its first sequence
+      int lo = 0, hi = groups_of(p.batch, stride);
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (prefix[mid] <= x) lo = mid;
         else hi = mid;
       }
-      b = lo;
+      b = lo * stride;
+      seq0 = prefix[lo];
+      seq_end = seq0 + sequence_steps<ROWS, PER>(p, b, G);
     }
-    while (prefix[b + 1] <= x) ++b;
-    int at = x - prefix[b], mt = 0, n;
+    while (seq_end <= x) {
+      ++b;
+      seq0 = seq_end;
+      seq_end += sequence_steps<ROWS, PER>(p, b, G);
+    }
+    int at = x - seq0, mt = 0, n;
+    Span s;
     for (;; ++mt) {
-      n = unit_steps<ROWS, PER>(p, b, mt, G, pc.s);
+      n = unit_steps<ROWS, PER>(p, b, mt, G, s);
       if (at < n * p.n_kv) break;
       at -= n * p.n_kv;
     }
+    pc.s = s;
     pc.b = b;
     pc.m0 = mt * ROWS;
     pc.kvh = at / n;
     const int s0 = at % n, s1 = min(n, s0 + (end - x));
-    const int tiles = (pc.s.hi - pc.s.lo + kKeys - 1) / kKeys;
+    const int tiles = (s.hi - s.lo + kKeys - 1) / kKeys;
     pc.t0 = s0 * PER;
     pc.nt = max(0, min(s1 * PER, tiles) - pc.t0);
     pc.whole = s0 == 0 && s1 == n;
-    pc.slot = 2 * cta + (first ? 0 : 1);
+    pc.slot = 2 * (int)blockIdx.x + (first ? 0 : 1);
     x += s1 - s0;
     first = false;
     return true;
   }
+};
+
+template <int ROWS, int PER>
+struct Misc {
+  static constexpr bool MT2 = PER == 1;
+  float2 ml[2][MT2 ? 1 : 128];  // key split: the warpgroups' (reference, sum) per row
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t s_full[2], p_full[2], pv_done[2], q_full[2];
+  unsigned bad[2][4];           // non-finite V rows of the tile at hand
+  uint32_t tmem;
+  int failed;
+  int prefix[kGroups + 1];      // first step of each group of sequences
+  Scan scan;
+  // What each warp works on.  In shared memory on purpose: a softmax thread's registers hold a row
+  // of scores, and values spilled to local memory would come from L2 (next to 200 KB of shared
+  // memory the L1 holds nothing for long), some 300 cycles each.
+  Piece pc[kThreads / 32];
+  Walk<ROWS, PER> walk[kThreads / 32];
 };
 
 // q . k of a row's head and the key at place j, in fp32, from global memory.
@@ -259,29 +346,29 @@ __device__ unsigned see_bits(const Params& p, const Span& s, int t, int pos, int
 }
 
 template <int HD, bool MT2, bool X2>
-__global__ void __launch_bounds__(kThreads, 1) tree_attn_t5_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 1)
+    tree_attn_t5_kernel(const __grid_constant__ Params p, const int stride) {
   using C = Cfg<HD, MT2, X2>;
   constexpr int PER = MT2 ? 1 : 2;  // key tiles per step
-  extern __shared__ uint8_t sm_raw[];
-  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
-  Misc& mi = *reinterpret_cast<Misc*>(sm + C::OFF_MISC);
+  extern __shared__ __align__(1024) uint8_t sm[];  // the kernel has no static shared memory
+  Misc<C::ROWS, PER>& mi = *reinterpret_cast<Misc<C::ROWS, PER>*>(sm + C::OFF_MISC);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.n_heads / p.n_kv;
 
   if (tid == 0) {
     for (int i = 0; i < C::SK; ++i) {
       mbar_init(&mi.k_full[i], 1);
-      mbar_init(&mi.k_empty[i], MT2 ? 2 : 1);
+      mbar_init(&mi.k_empty[i], 1);
     }
     for (int i = 0; i < C::SV; ++i) {
       mbar_init(&mi.v_full[i], 1);
-      mbar_init(&mi.v_empty[i], MT2 ? 2 : 1);
+      mbar_init(&mi.v_empty[i], 1);
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(&mi.s_full[g], 1);
-      mbar_init(&mi.p_full[g], 128);
+      mbar_init(&mi.p_full[g], 4);
       mbar_init(&mi.pv_done[g], 1);
-      mbar_init(&mi.q_full[g], MT2 ? 128 : 256);
+      mbar_init(&mi.q_full[g], MT2 ? 4 : 8);
       for (int w = 0; w < 4; ++w) mi.bad[g][w] = 0u;
     }
     mi.failed = 0;
@@ -293,16 +380,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_t5_kernel(const __grid_
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   fence_before();
-  steps_prefix<C::ROWS, PER>(p, G, mi.prefix, kThreads);
+  steps_prefix<C::ROWS, PER>(p, G, stride, mi.prefix, mi.scan);
   fence_after();
   const uint32_t tmem = mi.tmem;
-  const int W = mi.prefix[p.batch];
-  Walk<C::ROWS, PER> walk;
-  walk.x = part_begin(W, blockIdx.x, gridDim.x);
-  walk.end = part_begin(W, blockIdx.x + 1, gridDim.x);
-  walk.b = 0;
-  walk.first = true;
-  Piece pc;
+  const int W = mi.prefix[groups_of(p.batch, stride)];
+  Piece& pc = mi.pc[warp];
+  if (lane == 0) mi.walk[warp].begin(W);
+  auto next = [&]() { return mi.walk[warp].next(p, mi.prefix, stride, G, pc); };  // one lane
+  auto next_warp = [&]() {
+    __syncwarp();
+    bool more = false;
+    if (lane == 0) more = next();
+    more = __shfl_sync(0xffffffffu, (int)more, 0) != 0;
+    return more;
+  };
   bool dead = false;
   int kc = 0, vc = 0;  // tiles through the rings so far (every role counts them alike)
   auto wait = [&](uint64_t* bar, uint32_t phase) {
@@ -315,111 +406,145 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_t5_kernel(const __grid_
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    if (warp == 8) {
-      // ---------------- TMA: page loads, lane = page of the tile ----------------
-      while (!dead && walk.next(p, mi.prefix, G, blockIdx.x, pc)) {
+    if (warp == 8 || warp == 10) {
+      // ---------------- TMA: page loads of K (warp 8) or V (warp 10), lane = page of the tile ----
+      // A K page comes as HD/64 boxes of 16 rows x 128 bytes, each to its 64-column block of the
+      // tile; a V page as one box of all of them (the MMA takes a page per 16 keys of reduction).
+      const bool is_k = warp == 8;
+      const int stages = is_k ? C::SK : C::SV;
+      uint64_t* full = is_k ? mi.k_full : mi.v_full;
+      uint64_t* empty = is_k ? mi.k_empty : mi.v_empty;
+      while (!dead && next_warp()) {
         const int* bt = p.block_table + (long long)pc.b * p.max_blocks;
-        int page0 = pc.s.lo / 16 + pc.t0 * (kKeys / 16);
+        const int page0 = pc.s.lo / 16 + pc.t0 * (kKeys / 16);
         auto page_id = [&](int tile) {
           const int pg = page0 + tile * (kKeys / 16) + lane;
           const int id = (lane < kKeys / 16 && tile < pc.nt && pg < p.max_blocks && pg * 16 < pc.s.hi) ? bt[pg] : -1;
           return id >= 0 && id < p.n_blocks ? id : -1;
         };
         int id = page_id(0);
-        for (int i = 0; i < pc.nt && !dead; ++i, ++kc, ++vc) {
+        for (int i = 0; i < pc.nt; ++i, ++kc) {
           const int ahead = page_id(i + 1);
-          const unsigned have = __ballot_sync(0xffffffffu, id >= 0) & 0xffu;
-          const int row = (id * p.n_kv + pc.kvh) * 16;
-          const uint32_t bytes = __popc(have) * 16 * HD * 2;
-          const int ks = kc % C::SK, vs = vc % C::SV;
-          if (kc >= C::SK) wait(&mi.k_empty[ks], (kc / C::SK - 1) & 1);
+          const unsigned have = __ballot_sync(0xffffffffu, id >= 0);
+          const int row = (id * p.n_kv + pc.kvh) * 16, st = kc % stages;
+          if (kc >= stages) wait(&empty[st], (kc / stages - 1) & 1);
           dead = __any_sync(0xffffffffu, dead);
           if (dead) break;
           if (lane == 0) {
-            if (bytes) mbar_expect_tx(&mi.k_full[ks], bytes);
-            else mbar_arrive(&mi.k_full[ks]);
+            if (have) mbar_expect_tx(&full[st], __popc(have) * 16 * HD * 2);
+            else mbar_arrive(&full[st]);
           }
           __syncwarp();
-          if (id >= 0)
-  #pragma unroll
-            for (int bx = 0; bx < C::BOXES; ++bx)
-              tma_load_2d(sm + C::OFF_K + ks * C::TILE + bx * kKeys * 128 + lane * 2048, &p.tmK, bx * 64, row,
-                          &mi.k_full[ks]);
-          if (vc >= C::SV) wait(&mi.v_empty[vs], (vc / C::SV - 1) & 1);
-          dead = __any_sync(0xffffffffu, dead);
-          if (dead) {
-            ++kc;  // the K tile is in flight
-            break;
+          if (id >= 0) {
+            if (is_k) {
+#pragma unroll
+              for (int bx = 0; bx < C::BOXES; ++bx)
+                tma_load_2d(sm + C::OFF_K + st * C::TILE + bx * kKeys * 128 + lane * 2048, &p.tmK, bx * 64, row,
+                            &full[st]);
+            } else {
+              tma_load_3d(sm + C::OFF_V + st * C::TILE + lane * (HD * 32), &p.tmV, 0, row, 0, &full[st]);
+            }
           }
-          if (lane == 0) {
-            mi.miss[vs] = ~have & 0xffu;
-            if (bytes) mbar_expect_tx(&mi.v_full[vs], bytes);
-            else mbar_arrive(&mi.v_full[vs]);
-          }
-          __syncwarp();
-          if (id >= 0)
-  #pragma unroll
-            for (int bx = 0; bx < C::BOXES; ++bx)
-              tma_load_2d(sm + C::OFF_V + vs * C::TILE + bx * kKeys * 128 + lane * 2048, &p.tmV, bx * 64, row,
-                          &mi.v_full[vs]);
           id = ahead;
         }
       }
-    } else if (warp < 11) {
-      // ---------------- MMA: one warp per warpgroup, one lane of it ----------------
-      const int g = warp - 9;
-      if (lane == 0) {
-        const uint32_t s_col = tmem + g * 128, o_col = tmem + 256 + g * HD;
-        const uint32_t q = smem_u32(sm) + (MT2 ? g * C::TILE : 0);
-        int np = 0, nq = 0;  // PV products issued, pieces with tiles of this warpgroup
-        while (walk.next(p, mi.prefix, G, blockIdx.x, pc)) {
-          auto qk = [&](int i) {  // S = Q K^T of tile i of the piece
-            const int c = kc + i, ks = c % C::SK;
+      if (*reinterpret_cast<volatile int*>(&mi.failed)) {  // copies in flight land before the CTA ends
+        for (int i = max(0, kc - stages); i < kc; ++i) mbar_wait(&full[i % stages], (i / stages) & 1, &g_error, 1);
+      }
+    } else if (warp == 9) {
+      // ---------------- MMA: one elected lane, the warpgroups in turn ----------------
+      // A turn is P V of one warpgroup's tile and the scores of its next one, back to back: while the
+      // tensor cores do that, the other warpgroup has the exponential units to itself, and the two
+      // keep alternating.  (Two issuing threads let both warpgroups do the same thing at the same
+      // time: 275 us instead of TODO for 8 trees of 64 nodes over 8k-32k places.)
+      const uint32_t sm0 = smem_u32(sm);
+      int np[2] = {0, 0}, nq = 0;  // products issued per warpgroup, pieces begun
+      while (next_warp()) {
+        auto qk = [&](int g, int i, bool first, bool last) {  // S_g = Q_g K^T of tile i of the piece
+          const int c = kc + i, ks = c % C::SK;
+          if (first) {
             wait(&mi.k_full[ks], (c / C::SK) & 1);
             fence_after();
-            const uint32_t k = smem_u32(sm) + C::OFF_K + ks * C::TILE;
-  #pragma unroll
+          }
+          const uint32_t q = desc_k(sm0 + (MT2 ? g * C::TILE : 0)), k = desc_k(sm0 + C::OFF_K + ks * C::TILE);
+          if (elect_one()) {
+#pragma unroll
             for (int pl = 0; pl < (X2 ? 2 : 1); ++pl)
-  #pragma unroll
+#pragma unroll
               for (int e = 0; e < HD / 16; ++e) {
-                const uint32_t o = (e >> 2) * kKeys * 128 + (e & 3) * 32;
-                mma_ss(s_col, desc_k(q + pl * C::TILE + o), desc_k(k + o), idesc(kKeys, false), pl > 0 || e > 0);
+                const uint32_t o = ((e >> 2) * kKeys * 128 + (e & 3) * 32) >> 4;
+                mma_ss(tmem + g * 128, q + pl * (C::TILE >> 4) + o, k + o, idesc(kKeys, false), pl > 0 || e > 0);
               }
             commit(&mi.s_full[g]);
-            commit(&mi.k_empty[ks]);
-          };
-          constexpr int STEP = MT2 ? 1 : 2;
-          const int i0 = MT2 ? 0 : g;
-          if (i0 < pc.nt) {
-            wait(&mi.q_full[g], nq & 1);
-            ++nq;
-            fence_after();
-            qk(i0);
+            if (last) commit(&mi.k_empty[ks]);
           }
-          for (int i = i0; i < pc.nt; i += STEP) {
-            const int c = vc + i, vs = c % C::SV;
-            wait(&mi.v_full[vs], (c / C::SV) & 1);
-            wait(&mi.p_full[g], np & 1);
-            fence_after();
-            const uint32_t v = smem_u32(sm) + C::OFF_V + vs * C::TILE;
-  #pragma unroll
+          __syncwarp();
+        };
+        auto pv = [&](int g, int i, bool first, bool last) {  // O_g += P_g V of tile i
+          const int c = vc + i, vs = c % C::SV;
+          if (first) wait(&mi.v_full[vs], (c / C::SV) & 1);
+          wait(&mi.p_full[g], np[g] & 1);
+          fence_after();
+          const uint32_t v = desc_mn(sm0 + C::OFF_V + vs * C::TILE, 2048);
+          if (elect_one()) {
+#pragma unroll
             for (int pl = 0; pl < (X2 ? 2 : 1); ++pl)
-  #pragma unroll
+#pragma unroll
               for (int e = 0; e < kKeys / 16; ++e)
-                mma_ts(o_col, s_col + pl * 64 + e * 8, desc_mn(v + e * 2048, kKeys * 128), idesc(HD, true));
+                mma_ts(tmem + 256 + g * HD, tmem + g * 128 + pl * 64 + e * 8, v + e * (HD * 2), idesc(HD, true));
             commit(&mi.pv_done[g]);
-            commit(&mi.v_empty[vs]);
-            if (i + STEP < pc.nt) {
-              // the next scores overwrite the P this product reads
-              wait(&mi.pv_done[g], np & 1);
-              fence_after();
-              qk(i + STEP);
-            }
-            ++np;
+            if (last) commit(&mi.v_empty[vs]);
           }
-          kc += pc.nt;
-          vc += pc.nt;
+          __syncwarp();
+        };
+        auto pv_wait = [&](int g) {  // the next scores overwrite the P that the product reads
+          wait(&mi.pv_done[g], np[g] & 1);
+          fence_after();
+        };
+        wait(&mi.q_full[0], nq & 1);
+        if (MT2) wait(&mi.q_full[1], nq & 1);
+        ++nq;
+        fence_after();
+        if constexpr (MT2) {
+          qk(0, 0, true, false);
+          qk(1, 0, false, true);
+          for (int i = 0; i < pc.nt; ++i) {
+            const bool more = i + 1 < pc.nt;
+            pv(0, i, true, false);
+            if (more) {
+              pv_wait(0);
+              qk(0, i + 1, true, false);
+            }
+            ++np[0];
+            pv(1, i, false, true);
+            if (more) {
+              pv_wait(1);
+              qk(1, i + 1, false, true);
+            }
+            ++np[1];
+          }
+        } else {
+          qk(0, 0, true, true);
+          if (pc.nt > 1) qk(1, 1, true, true);
+          for (int i = 0; i < pc.nt; i += 2) {
+            pv(0, i, true, true);
+            if (i + 2 < pc.nt) {
+              pv_wait(0);
+              qk(0, i + 2, true, true);
+            }
+            ++np[0];
+            if (i + 1 < pc.nt) {
+              pv(1, i + 1, true, true);
+              if (i + 3 < pc.nt) {
+                pv_wait(1);
+                qk(1, i + 3, true, true);
+              }
+              ++np[1];
+            }
+          }
         }
+        kc += pc.nt;
+        vc += pc.nt;
       }
     }
   } else {
@@ -429,29 +554,40 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_t5_kernel(const __grid_
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane of the warp's first row
     const uint32_t s_col = tmem + lanes + g * 128, o_col = tmem + lanes + 256 + g * HD;
     int ns = 0;  // score tiles of this warpgroup so far
-    while (walk.next(p, mi.prefix, G, blockIdx.x, pc)) {
+    while (next_warp()) {
       const Span& s = pc.s;
       const int m = pc.m0 + (MT2 ? g * 128 : 0) + r, t = m / G, head = pc.kvh * G + m % G;
       const bool live = t < s.T;
       const int pos = live ? row_position(p, s, t) : s.ctx;
       const bool warp_live = __any_sync(0xffffffffu, live);
       // Q rows into shared memory: MT2, own tile; key split, half of the one tile each
-      for (int x = (MT2 ? r : tid); x < 128 * (HD / 8); x += MT2 ? 128 : 256) {
-        const int rr = x / (HD / 8), ch = x % (HD / 8);
-        const int mm = pc.m0 + (MT2 ? g * 128 : 0) + rr, tt = mm / G;
-        uint4 h = make_uint4(0u, 0u, 0u, 0u), l = h;
-        if (tt < s.T) q_chunk(p, s.row0 + tt, pc.kvh * G + mm % G, HD, ch, h, l);
-        uint8_t* dst = sm + (MT2 ? g * C::TILE : 0) + sw(rr, ch, 128);
-        *reinterpret_cast<uint4*>(dst) = h;
-        if (X2) *reinterpret_cast<uint4*>(dst + C::TILE) = l;
+      constexpr int QN = MT2 ? 128 : 256, QI = 128 * (HD / 8) / QN;
+      uint8_t* qt = sm + (MT2 ? g * C::TILE : 0);
+      const int qm = pc.m0 + (MT2 ? g * 128 : 0), qx = MT2 ? r : tid;
+      if (p.q_f16) {
+#pragma unroll
+        for (int it = 0; it < QI; ++it) {
+          const int x = it * QN + qx, rr = x / (HD / 8), ch = x % (HD / 8), mm = qm + rr, tt = mm / G;
+          const bool ok = tt < s.T;
+          const long long at =
+              ok ? (long long)(s.row0 + tt) * p.ldq + (long long)(pc.kvh * G + mm % G) * HD + ch * 8 : 0;
+          cp_async16(qt + sw(rr, ch, 128), static_cast<const uint16_t*>(p.q) + at, ok);
+          if (X2) *reinterpret_cast<uint4*>(qt + C::TILE + sw(rr, ch, 128)) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+      } else {
+#pragma unroll 2
+        for (int it = 0; it < QI; ++it) {
+          const int x = it * QN + qx, rr = x / (HD / 8), ch = x % (HD / 8), mm = qm + rr, tt = mm / G;
+          uint4 h = make_uint4(0u, 0u, 0u, 0u), l = h;
+          if (tt < s.T) q_chunk(p, s.row0 + tt, pc.kvh * G + mm % G, HD, ch, h, l);
+          *reinterpret_cast<uint4*>(qt + sw(rr, ch, 128)) = h;
+          if (X2) *reinterpret_cast<uint4*>(qt + C::TILE + sw(rr, ch, 128)) = l;
+        }
       }
       fence_async();
-      if constexpr (MT2) {
-        mbar_arrive(&mi.q_full[g]);
-      } else {  // an MMA warp hears of the pieces that have a tile for it
-        mbar_arrive(&mi.q_full[0]);
-        if (pc.nt > 1) mbar_arrive(&mi.q_full[1]);
-      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&mi.q_full[MT2 ? g : 0]);
       {  // O starts at zero: every product adds to it
         uint32_t z[32];
 #pragma unroll
@@ -461,22 +597,36 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_t5_kernel(const __grid_
         tmem_wait_st();
       }
       float ref = -INFINITY, sum = 0.f;
+      // pages of a tile that do not exist (the TMA warp skips them): lanes 0-7 look one tile ahead
+      auto page_ok = [&](int tile) {
+        const int pg = s.lo / 16 + (pc.t0 + tile) * (kKeys / 16) + lane;
+        if (lane >= kKeys / 16 || tile >= pc.nt || pg >= p.max_blocks || pg * 16 >= s.hi) return false;
+        const int id = p.block_table[(long long)pc.b * p.max_blocks + pg];
+        return id >= 0 && id < p.n_blocks;
+      };
+      bool have = page_ok(MT2 ? 0 : g);
 
       for (int i = MT2 ? 0 : g; i < pc.nt; i += PER) {
         const int c = vc + i, vs = c % C::SV, j0 = s.lo + (pc.t0 + i) * kKeys;
-        wait(&mi.v_full[vs], (c / C::SV) & 1);
-        const unsigned miss = mi.miss[vs];
+        const unsigned miss = ~__ballot_sync(0xffffffffu, have) & 0xffu;
+        have = page_ok(i + PER);
         const bool whole = miss == 0 && j0 + kKeys <= s.ctx && (p.window == 0 || j0 > s.pmax - p.window);
+        // the scores being there, this warpgroup's last product is done: its V stage has turned over,
+        // and a wait for the next tile in it cannot mistake the phase
+        wait(&mi.s_full[g], ns & 1);
+        ++ns;
+        fence_after();
         unsigned bad[4] = {0u, 0u, 0u, 0u};
         if (!whole) {
           // zero the V rows past the end or without a page, find and zero non-finite ones; MT2
           // shares the tile, and the two warpgroups do half each
+          wait(&mi.v_full[vs], (c / C::SV) & 1);
           uint8_t* V = sm + C::OFF_V + vs * C::TILE;
           const int id = MT2 ? 3 : 1 + g, n = MT2 ? 256 : 128, me = MT2 ? tid : r;
           unsigned* flags = mi.bad[MT2 ? 0 : g];
           for (int x = me; x < kKeys * (HD / 8); x += n) {
             const int rr = x / (HD / 8), ch = x % (HD / 8);
-            uint4* v = reinterpret_cast<uint4*>(V + sw(rr, ch, kKeys));
+            uint4* v = reinterpret_cast<uint4*>(V + v_at<HD>(rr, ch));
             if (j0 + rr >= s.hi || ((miss >> (rr >> 4)) & 1)) {
               *v = make_uint4(0u, 0u, 0u, 0u);
             } else if (nonfinite(*v)) {
@@ -491,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_t5_kernel(const __grid_
             for (int x = me; x < kKeys * (HD / 8); x += n) {
               const int rr = x / (HD / 8), ch = x % (HD / 8);
               if ((bad[rr >> 5] >> (rr & 31)) & 1)
-                *reinterpret_cast<uint4*>(V + sw(rr, ch, kKeys)) = make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4*>(V + v_at<HD>(rr, ch)) = make_uint4(0u, 0u, 0u, 0u);
             }
             fence_async();
             bar_sync(id, n);
@@ -499,24 +649,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_t5_kernel(const __grid_
             bar_sync(id, n);
           }
         }
-        wait(&mi.s_full[g], ns & 1);
-        ++ns;
-        fence_after();
         if (warp_live) {
+          unsigned see[4];  // formed before the scores fill the registers
+          if (!whole) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              see[w] = live ? see_bits(p, s, t, pos, j0 + 32 * w) : 0u;
+              if ((miss >> (2 * w)) & 1) see[w] &= 0xffff0000u;
+              if ((miss >> (2 * w + 1)) & 1) see[w] &= 0x0000ffffu;
+            }
+          }
           float x[kKeys];
 #pragma unroll
           for (int e = 0; e < kKeys; e += 32) tmem_ld32(s_col + e, reinterpret_cast<uint32_t*>(x) + e);
           tmem_wait_ld();
           if (!whole) {  // places the row does not see, whatever they hold
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              unsigned see = live ? see_bits(p, s, t, pos, j0 + 32 * w) : 0u;
-              if ((miss >> (2 * w)) & 1) see &= 0xffff0000u;
-              if ((miss >> (2 * w + 1)) & 1) see &= 0x0000ffffu;
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!((see >> e) & 1u)) x[32 * w + e] = -INFINITY;
-            }
+            for (int e = 0; e < kKeys; ++e)
+              if (!((see[e >> 5] >> (e & 31)) & 1u)) x[e] = -INFINITY;
           }
           if constexpr (X2) {
             // hi + lo parts make NaN of an infinite k where the product itself is fine
@@ -536,10 +686,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_t5_kernel(const __grid_
               }
             }
           }
-          float mx = x[0];
+          float m4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-          for (int e = 1; e < kKeys; ++e) mx = fmaxf(mx, x[e]);
-          mx *= p.scale_log2;
+          for (int e = 4; e < kKeys; e += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              m4[k] = e + 4 + k < kKeys ? fmaxf(fmaxf(m4[k], x[e + k]), x[e + 4 + k]) : fmaxf(m4[k], x[e + k]);
+          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
           const bool grow = mx > ref + kSlack || (ref == -INFINITY && mx > -INFINITY);
           if (__any_sync(0xffffffffu, grow)) {
             const float to = grow ? mx : ref;
@@ -559,44 +712,51 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_t5_kernel(const __grid_
             }
           }
           const float base = ref == -INFINITY ? 0.f : ref;  // nothing seen yet: weights 2^-inf
-          float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-          for (int e = 0; e < kKeys; e += 2) {
-            x[e] = ex2(fmaf(x[e], p.scale_log2, -base));
-            x[e + 1] = ex2(fmaf(x[e + 1], p.scale_log2, -base));
-            s0 += x[e];
-            s1 += x[e + 1];
-          }
-          sum += s0 + s1;
           // weights as fp16 over the scores: relative 2^-11, the output's own rounding; with X2
           // their remainders behind them
+          const uint64_t c2 = two(p.scale_log2, p.scale_log2), b2 = two(-base, -base);
+          uint64_t acc[2] = {0ull, 0ull};
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t w[32];
+          for (int h = 0; h < 4; ++h) {
+            uint32_t w[16];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) w[e] = pack2(x[64 * h + 2 * e], x[64 * h + 2 * e + 1]);
-            tmem_st32(s_col + 32 * h, w);
+            for (int e = 0; e < 16; ++e) {
+              float& x0 = x[32 * h + 2 * e];
+              float& x1 = x[32 * h + 2 * e + 1];
+              const float2 z = split(fma2(two(x0, x1), c2, b2));
+              x0 = ex2(z.x);
+              x1 = ex2(z.y);
+              acc[e & 1] = add2(acc[e & 1], two(x0, x1));
+              w[e] = pack2(x0, x1);
+            }
+            tmem_st16(s_col + 16 * h, w);
             if constexpr (X2) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) w[e] = pack2_rest(x[64 * h + 2 * e], x[64 * h + 2 * e + 1], w[e]);
-              tmem_st32(s_col + 64 + 32 * h, w);
+              for (int e = 0; e < 16; ++e) w[e] = pack2_rest(x[32 * h + 2 * e], x[32 * h + 2 * e + 1], w[e]);
+              tmem_st16(s_col + 64 + 16 * h, w);
             }
           }
+          const float2 s01 = split(add2(acc[0], acc[1]));
+          sum += s01.x + s01.y;
           if (bad[0] | bad[1] | bad[2] | bad[3]) {  // non-finite V rows: the rows that see them alone
             tmem_wait_st();
 #pragma unroll 1
             for (int k = 0; k < kKeys; ++k) {
               if (!((bad[k >> 5] >> (k & 31)) & 1u)) continue;
-              float w = 0.f;
-#pragma unroll
-              for (int e = 0; e < kKeys; ++e) take_if(w, x[e], e, k);
+              const float2 w2 = h2f2(tmem_ld1(s_col + k / 2));
+              float w = (k & 1) ? w2.y : w2.x;
+              if constexpr (X2) {
+                const float2 l2 = h2f2(tmem_ld1(s_col + 64 + k / 2));
+                w += (k & 1) ? l2.y : l2.x;
+              }
               add_place<HD>(p, pc.b, pc.kvh, j0 + k, w, o_col);
             }
           }
           tmem_wait_st();
         }
         fence_before();
-        mbar_arrive(&mi.p_full[g]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&mi.p_full[g]);
       }
       kc += pc.nt;
       vc += pc.nt;
@@ -662,26 +822,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_t5_kernel(const __grid_
   fence_before();
   __syncthreads();
   fence_after();
-  if (mi.failed && warp == 8 && lane == 0) {  // copies in flight land before the CTA ends
-    for (int i = max(0, kc - C::SK); i < kc; ++i) mbar_wait(&mi.k_full[i % C::SK], (i / C::SK) & 1, &g_error, 1);
-    for (int i = max(0, vc - C::SV); i < vc; ++i) mbar_wait(&mi.v_full[i % C::SV], (i / C::SV) & 1, &g_error, 1);
-  }
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
 }
 
 // Joins the pieces of each unit that more than one CTA worked on; one warp per row.
 template <int HD, int ROWS, int PER>
-__global__ void __launch_bounds__(256) tree_join_t5_kernel(const Params p, int ctas) {
-  __shared__ int prefix[kMaxBatch + 1];
+__global__ void __launch_bounds__(256) tree_join_t5_kernel(const Params p, int ctas, int stride) {
+  __shared__ int prefix[kGroups + 1];
+  __shared__ Scan scan;
   const int G = p.n_heads / p.n_kv;
   const int b = blockIdx.z, mt = blockIdx.y / p.n_kv, kvh = blockIdx.y % p.n_kv;
   Span s;
   const int n = unit_steps<ROWS, PER>(p, b, mt, G, s);
   if (n == 0) return;
-  steps_prefix<ROWS, PER>(p, G, prefix, 256);
-  const int W = prefix[p.batch];
-  int u0 = prefix[b];
+  steps_prefix<ROWS, PER>(p, G, stride, prefix, scan);
+  const int W = prefix[groups_of(p.batch, stride)];
+  int u0 = prefix[b / stride];
+  for (int i = b / stride * stride; i < b; ++i) u0 += sequence_steps<ROWS, PER>(p, i, G);
   for (int i = 0; i < mt; ++i) {
     Span q;
     u0 += p.n_kv * unit_steps<ROWS, PER>(p, b, i, G, q);
@@ -726,15 +884,15 @@ __global__ void __launch_bounds__(256) tree_join_t5_kernel(const Params p, int c
 }
 
 // Whether this kernel serves the call (the other one has no limits of this kind).
-static bool serves(int head_dim, int batch, long long max_steps) {
-  return (head_dim == 64 || head_dim == 128) && batch <= kMaxBatch && max_steps < (1ll << 31);
+static bool serves(int head_dim, long long max_steps) {
+  return (head_dim == 64 || head_dim == 128) && max_steps < (1ll << 31);
 }
 
 // Rows of a unit, key tiles per step.  256 rows where a sequence may fill more than 128 (each K/V
 // tile then serves two row tiles), unless hi + lo planes need the room.
 struct Shape {
   bool mt2;
-  int rows, m_tiles, grid;
+  int rows, m_tiles, grid, stride;
   long long max_steps;
   size_t off_ml, bytes;
 };
@@ -747,6 +905,7 @@ static Shape shape_of(int batch, int n_heads, int n_kv, int head_dim, int max_q,
   const int keys = h.mt2 ? kKeys : 2 * kKeys;
   // + 1: with a window, a unit's first tile may begin anywhere
   h.max_steps = (long long)batch * n_kv * h.m_tiles * ((max_ctx + keys - 1) / keys + 1);
+  h.stride = (batch + kGroups - 1) / kGroups;
   h.grid = (int)std::min<long long>(num_sms(), h.max_steps);
   h.off_ml = (size_t)2 * h.grid * h.rows * head_dim * sizeof(float);
   h.bytes = h.off_ml + (size_t)2 * h.grid * h.rows * 2 * sizeof(float);
@@ -757,17 +916,18 @@ template <int HD, bool MT2, bool X2>
 static int launch(Params& p, const Shape& h, cudaStream_t stream) {
   using C = Cfg<HD, MT2, X2>;
   auto kern = tree_attn_t5_kernel<HD, MT2, X2>;
-  const int smem = C::OFF_MISC + (int)sizeof(Misc) + 1024;
+  const int smem = C::OFF_MISC + (int)sizeof(Misc<C::ROWS, MT2 ? 1 : 2>);
+  static_assert(C::OFF_MISC + sizeof(Misc<C::ROWS, MT2 ? 1 : 2>) <= 227 * 1024, "shared memory of one CTA");
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
     set_cuda_error(e);
     cudaGetLastError();
     return B2D_ERR_CUDA;
   }
-  kern<<<h.grid, kThreads, smem, stream>>>(p);
+  kern<<<h.grid, kThreads, smem, stream>>>(p, h.stride);
   B2D_TRY(launch_status());
   tree_join_t5_kernel<HD, C::ROWS, MT2 ? 1 : 2>
-      <<<dim3(C::ROWS / 32, h.m_tiles * p.n_kv, p.batch), 256, 0, stream>>>(p, h.grid);
+      <<<dim3(C::ROWS / 32, h.m_tiles * p.n_kv, p.batch), 256, 0, stream>>>(p, h.grid, h.stride);
   return launch_status();
 }
 
