@@ -956,6 +956,22 @@ int make_tmap_f16_blocks(CUtensorMap* m, const void* base, uint64_t rows, int co
   return r == CUDA_SUCCESS ? B2D_OK : B2D_ERR_ALIGN;
 }
 
+// fp16 [rows (stride ld), heads, hd] as 64-column blocks: box {64 columns, box_heads, box_rows, 1},
+// its rows in the order (row, head).
+int make_tmap_f16_heads(CUtensorMap* m, const void* base, uint64_t rows, int heads, int hd, int ld, int box_heads,
+                        int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return B2D_ERR_CUDA;
+  cuuint64_t dims[4] = {64, (cuuint64_t)heads, (cuuint64_t)rows, (cuuint64_t)hd / 64};
+  cuuint64_t strides[3] = {(cuuint64_t)hd * 2, (cuuint64_t)ld * 2, 128};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides,
+                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? B2D_OK : B2D_ERR_ALIGN;
+}
+
 // 2D uint8 tensor [rows, cols] (bytes), box {box_cols, box_rows}, no swizzle: the raw tiles of
 // quantized weights, which the dequant warps read with plain shared-memory loads.
 static int make_tmap_u8(CUtensorMap* m, const void* base, uint64_t rows, int cols, int box_cols,

@@ -33,6 +33,8 @@ namespace b2d {
 
 int make_tmap_f16(CUtensorMap* m, const void* base, uint64_t rows, int cols, int ld, int box_rows);
 int make_tmap_f16_blocks(CUtensorMap* m, const void* base, uint64_t rows, int cols, int box_rows);
+int make_tmap_f16_heads(CUtensorMap* m, const void* base, uint64_t rows, int heads, int hd, int ld, int box_heads,
+                        int box_rows);
 
 namespace tree {
 
@@ -49,6 +51,7 @@ struct Params {
   // page pools as [n_blocks * Hkv * 16, HD] fp16: boxes of 64 columns x 16 rows (tcgen05 kernel's V:
   // 16 rows x all 64-column blocks)
   CUtensorMap tmK, tmV;
+  CUtensorMap tmQ;  // q rows as [64-column block][row][head]: G heads x 128 / G rows per box
   const void* q;
   int q_f16;
   long long ldq;
@@ -161,9 +164,8 @@ __device__ __forceinline__ void consumers_sync() {
   asm volatile("bar.sync 1, 128;" ::: "memory");
 }
 
-// 8 elements of a q row as fp16, and what fp32 elements have beyond that.
-__device__ __forceinline__ void q_chunk(const Params& p, int row, int head, int hd, int ch, uint4& h, uint4& l) {
-  const long long at = (long long)row * p.ldq + (long long)head * hd + ch * 8;
+// 8 elements of q from element `at` on as fp16, and what fp32 elements have beyond that.
+__device__ __forceinline__ void q_chunk(const Params& p, long long at, uint4& h, uint4& l) {
   if (p.q_f16) {
     h = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at);
   } else {
@@ -176,11 +178,9 @@ __device__ __forceinline__ void q_chunk(const Params& p, int row, int head, int 
 }
 // Any of 8 fp16 values infinite or NaN.
 __device__ __forceinline__ bool nonfinite(uint4 u) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-  bool any = false;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) any |= (w[e] & 0x7c00u) == 0x7c00u || (w[e] & 0x7c000000u) == 0x7c000000u;
-  return any;
+  // an exponent of all ones, and only that, carries into the sign's place
+  auto carry = [](uint32_t w) { return (w & 0x7c007c00u) + 0x04000400u; };
+  return ((carry(u.x) | carry(u.y) | carry(u.z) | carry(u.w)) & 0x80008000u) != 0;
 }
 
 // 32 consecutive output elements from i on (16-byte aligned).
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
     const int r = i / (HD / 8), ch = i % (HD / 8);
     const int m = m0 + r, t = m / G, g = m % G;
     uint4 h = make_uint4(0u, 0u, 0u, 0u), l = h;
-    if (t < s.T) q_chunk(p, s.row0 + t, kvh * G + g, HD, ch, h, l);
+    if (t < s.T) q_chunk(p, (long long)(s.row0 + t) * p.ldq + (long long)(kvh * G + g) * HD + ch * 8, h, l);
     *reinterpret_cast<uint4*>(qs + sw(r, ch, kRows)) = h;
     if (X2) *reinterpret_cast<uint4*>(qs + C::Q_PLANE + sw(r, ch, kRows)) = l;
   }
@@ -716,6 +716,9 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
   const tree::t5::Shape h = tree::t5::shape_of(batch, n_heads, n_kv_heads, head_dim, max_q, max_ctx, x2);
   if (tree::t5::serves(head_dim, h.max_steps)) {
     B2D_TRY(make_tmap_f16_blocks(&p.tmV, v_pages, prows, head_dim, 16));
+    const int G = n_heads / n_kv_heads;
+    if (p.q_f16 && 128 % G == 0)
+      B2D_TRY(make_tmap_f16_heads(&p.tmQ, q, rows, n_heads, head_dim, ldq, G, 128 / G));
     p.m_tiles = h.m_tiles;
     p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + h.off_ml);
     if (head_dim == 64)

@@ -17,7 +17,7 @@
 //   key split: they hold the same 128 rows and take alternate key tiles; their two states meet
 //   through TMEM at the end of the unit.
 // Roles: warps 0-7 softmax (warp w reads TMEM lanes 32 (w % 4) ..), warps 8 and 10 load K and V
-// (TMA), warp 9 issues the MMAs.
+// (TMA), warp 9 issues the MMAs, warp 11 loads the next unit's Q while this one ends.
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the last time (its
 // weights are then up to 256 and still exact to 2^-11 in fp16), which after the first tiles of a
@@ -33,7 +33,7 @@ namespace t5 {
 
 constexpr int kKeys = 128;
 constexpr int kSoftmax = 256;               // threads of the two warpgroups
-constexpr int kThreads = kSoftmax + 128;    // + K, V and MMA warps, one idle
+constexpr int kThreads = kSoftmax + 128;    // + K, MMA, V and Q warps
 // Registers: a softmax thread holds a row of 128 scores.  384 threads launch with 168 each
 // (64512); the split 256 * 224 + 128 * 56 uses the same number.
 constexpr int kRegsSoftmax = 224, kRegsOther = 56;
@@ -97,10 +97,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {  // zeros if not
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0)
-               : "memory");
-}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -115,6 +111,13 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* tm, in
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* tm, int c0, int c1, int c2, int c3, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
       : "memory");
 }
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
@@ -227,43 +230,40 @@ __device__ __forceinline__ int part_begin(int W, int cta, int ctas) { return (in
 // Walks the pieces of steps [x, end) of the line.
 template <int ROWS, int PER>
 struct Walk {
-  int x, end, b, seq0, seq_end;  // sequence b holds steps [seq0, seq_end)
+  int x, end;
+  int b, mt, n, at0;  // the units of row tile mt of sequence b, n steps each, begin at step at0
   bool first;
-  __device__ void begin(int W) {
+  __device__ void begin(const Params& p, const int* prefix, int stride, int W) {
     x = part_begin(W, blockIdx.x, gridDim.x);
     end = part_begin(W, blockIdx.x + 1, gridDim.x);
     first = true;
+    int lo = 0, hi = groups_of(p.batch, stride);  // the group of sequences that holds step x
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] <= x) lo = mid;
+      else hi = mid;
+    }
+    b = lo * stride - 1;  // the first call of next() goes on to the next sequence
+    mt = p.m_tiles;
+    n = 0;
+    at0 = prefix[lo];
   }
-  __device__ bool next(const Params& p, const int* prefix, int stride, int G, Piece& pc) {
+  __device__ bool next(const Params& p, int G, Piece& pc) {
     if (x >= end) return false;
-    if (first) {  // the group of sequences that holds step x, and its first sequence
-      int lo = 0, hi = groups_of(p.batch, stride);
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (prefix[mid] <= x) lo = mid;
-        else hi = mid;
+    Span s = pc.s;
+    while (x >= at0 + n * p.n_kv) {  // on to the units of the next row tile, or sequence
+      at0 += n * p.n_kv;
+      n = ++mt < p.m_tiles ? unit_steps<ROWS, PER>(p, b, mt, G, s) : 0;
+      if (n == 0) {
+        mt = 0;
+        n = unit_steps<ROWS, PER>(p, ++b, 0, G, s);
       }
-      b = lo * stride;
-      seq0 = prefix[lo];
-      seq_end = seq0 + sequence_steps<ROWS, PER>(p, b, G);
-    }
-    while (seq_end <= x) {
-      ++b;
-      seq0 = seq_end;
-      seq_end += sequence_steps<ROWS, PER>(p, b, G);
-    }
-    int at = x - seq0, mt = 0, n;
-    Span s;
-    for (;; ++mt) {
-      n = unit_steps<ROWS, PER>(p, b, mt, G, s);
-      if (at < n * p.n_kv) break;
-      at -= n * p.n_kv;
     }
     pc.s = s;
     pc.b = b;
     pc.m0 = mt * ROWS;
-    pc.kvh = at / n;
-    const int s0 = at % n, s1 = min(n, s0 + (end - x));
+    pc.kvh = (x - at0) / n;
+    const int s0 = x - at0 - pc.kvh * n, s1 = min(n, s0 + (end - x));
     const int tiles = (s.hi - s.lo + kKeys - 1) / kKeys;
     pc.t0 = s0 * PER;
     pc.nt = max(0, min(s1 * PER, tiles) - pc.t0);
@@ -280,8 +280,8 @@ struct Misc {
   static constexpr bool MT2 = PER == 1;
   float2 ml[2][MT2 ? 1 : 128];  // key split: the warpgroups' (reference, sum) per row
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
-  uint64_t s_full[2], p_full[2], pv_done[2], q_full[2];
-  unsigned bad[2][4];           // non-finite V rows of the tile at hand
+  uint64_t s_full[2], p_full[2], pv_done[2], q_full, q_empty, v_seen[2];
+  unsigned bad[2][3][4];        // non-finite V rows of a tile that was looked over
   uint32_t tmem;
   int failed;
   int prefix[kGroups + 1];      // first step of each group of sequences
@@ -317,6 +317,18 @@ __device__ __forceinline__ void add_place(const Params& p, int b, int kvh, int j
     tmem_st32(o_col + c, o);
   }
   tmem_wait_st();
+}
+
+// Whether the page of lane 0-7 of a tile exists (the V loader skips it otherwise).
+__device__ __forceinline__ bool page_exists(const Params& p, const Piece& pc, int tile, int lane) {
+  const int pg = pc.s.lo / 16 + (pc.t0 + tile) * (kKeys / 16) + lane;
+  if (lane >= kKeys / 16 || tile >= pc.nt || pg >= p.max_blocks || pg * 16 >= pc.s.hi) return false;
+  const int id = p.block_table[(long long)pc.b * p.max_blocks + pg];
+  return id >= 0 && id < p.n_blocks;
+}
+// Whether every row sees every place of the tile from j0 on.
+__device__ __forceinline__ bool whole_tile(const Params& p, const Span& s, int j0, unsigned miss) {
+  return miss == 0 && j0 + kKeys <= s.ctx && (p.window == 0 || j0 > s.pmax - p.window);
 }
 
 // Bits of the places k0 .. k0 + 31 that row t (of the sequence's own rows, at position pos) sees,
@@ -355,6 +367,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.n_heads / p.n_kv;
 
+  // fp16 rows whose heads fill a 128-row tile exactly come by TMA; others the softmax warps load
+  const bool q_tma = p.q_f16 && 128 % G == 0;
+
   if (tid == 0) {
     for (int i = 0; i < C::SK; ++i) {
       mbar_init(&mi.k_full[i], 1);
@@ -368,9 +383,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&mi.s_full[g], 1);
       mbar_init(&mi.p_full[g], 4);
       mbar_init(&mi.pv_done[g], 1);
-      mbar_init(&mi.q_full[g], MT2 ? 4 : 8);
-      for (int w = 0; w < 4; ++w) mi.bad[g][w] = 0u;
+      mbar_init(&mi.v_seen[g], MT2 ? 8 : 4);
+      for (int w = 0; w < 12; ++w) mi.bad[g][0][w] = 0u;
     }
+    mbar_init(&mi.q_full, q_tma ? 1 : 8);
+    mbar_init(&mi.q_empty, 1);
     mi.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -379,18 +396,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                  "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  if (X2 && q_tma) {  // an fp16 q has nothing beyond its high part
+    for (int x = tid; x < C::TILE / 16; x += kThreads)
+      *reinterpret_cast<uint4*>(sm + C::TILE + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+    fence_async();
+  }
   fence_before();
   steps_prefix<C::ROWS, PER>(p, G, stride, mi.prefix, mi.scan);
   fence_after();
   const uint32_t tmem = mi.tmem;
   const int W = mi.prefix[groups_of(p.batch, stride)];
   Piece& pc = mi.pc[warp];
-  if (lane == 0) mi.walk[warp].begin(W);
-  auto next = [&]() { return mi.walk[warp].next(p, mi.prefix, stride, G, pc); };  // one lane
+  if (lane == 0) mi.walk[warp].begin(p, mi.prefix, stride, W);
   auto next_warp = [&]() {
     __syncwarp();
     bool more = false;
-    if (lane == 0) more = next();
+    if (lane == 0) more = mi.walk[warp].next(p, G, pc);
     more = __shfl_sync(0xffffffffu, (int)more, 0) != 0;
     return more;
   };
@@ -459,6 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // time: 275 us instead of TODO for 8 trees of 64 nodes over 8k-32k places.)
       const uint32_t sm0 = smem_u32(sm);
       int np[2] = {0, 0}, nq = 0;  // products issued per warpgroup, pieces begun
+      int ns[2] = {0, 0};          // tiles looked over per warpgroup (MT2: ns[0])
       while (next_warp()) {
         auto qk = [&](int g, int i, bool first, bool last) {  // S_g = Q_g K^T of tile i of the piece
           const int c = kc + i, ks = c % C::SK;
@@ -480,9 +502,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
         };
+        bool have = page_exists(p, pc, 0, lane);
+        auto miss_at = [&](int i) {  // called for tile 0, 1, ...; looks one ahead
+          const unsigned m = ~__ballot_sync(0xffffffffu, have) & 0xffu;
+          have = page_exists(p, pc, i + 1, lane);
+          return m;
+        };
         auto pv = [&](int g, int i, bool first, bool last) {  // O_g += P_g V of tile i
           const int c = vc + i, vs = c % C::SV;
-          if (first) wait(&mi.v_full[vs], (c / C::SV) & 1);
+          if (first) {
+            wait(&mi.v_full[vs], (c / C::SV) & 1);
+            if (!whole_tile(p, pc.s, pc.s.lo + (pc.t0 + i) * kKeys, miss_at(i))) wait(&mi.v_seen[MT2 ? 0 : g], ns[g]++ & 1);
+          }
           wait(&mi.p_full[g], np[g] & 1);
           fence_after();
           const uint32_t v = desc_mn(sm0 + C::OFF_V + vs * C::TILE, 2048);
@@ -501,13 +532,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           wait(&mi.pv_done[g], np[g] & 1);
           fence_after();
         };
-        wait(&mi.q_full[0], nq & 1);
-        if (MT2) wait(&mi.q_full[1], nq & 1);
+        wait(&mi.q_full, nq & 1);
         ++nq;
+        // the first scores overwrite the last unit's weights
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (np[g] > 0) wait(&mi.pv_done[g], (np[g] - 1) & 1);
         fence_after();
+        auto q_done = [&]() {  // every score of the unit is on its way: Q may go once they are formed
+          if (elect_one()) commit(&mi.q_empty);
+          __syncwarp();
+        };
         if constexpr (MT2) {
           qk(0, 0, true, false);
           qk(1, 0, false, true);
+          if (pc.nt == 1) q_done();
           for (int i = 0; i < pc.nt; ++i) {
             const bool more = i + 1 < pc.nt;
             pv(0, i, true, false);
@@ -520,32 +559,47 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (more) {
               pv_wait(1);
               qk(1, i + 1, false, true);
+              if (i + 2 == pc.nt) q_done();
             }
             ++np[1];
           }
         } else {
           qk(0, 0, true, true);
           if (pc.nt > 1) qk(1, 1, true, true);
-          for (int i = 0; i < pc.nt; i += 2) {
-            pv(0, i, true, true);
-            if (i + 2 < pc.nt) {
-              pv_wait(0);
-              qk(0, i + 2, true, true);
-            }
-            ++np[0];
-            if (i + 1 < pc.nt) {
-              pv(1, i + 1, true, true);
-              if (i + 3 < pc.nt) {
-                pv_wait(1);
-                qk(1, i + 3, true, true);
+          if (pc.nt <= 2) q_done();
+          for (int i0 = 0; i0 < pc.nt; i0 += 2)
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const int i = i0 + g;
+              if (i >= pc.nt) break;
+              pv(g, i, true, true);
+              if (i + 2 < pc.nt) {
+                pv_wait(g);
+                qk(g, i + 2, true, true);
+                if (i + 3 == pc.nt) q_done();
               }
-              ++np[1];
+              ++np[g];
             }
-          }
         }
         kc += pc.nt;
         vc += pc.nt;
       }
+    } else if (q_tma) {
+      // ---------------- TMA: Q, as soon as the scores of the unit before are formed ----------------
+      int nq = 0;
+      while (next_warp()) {
+        if (nq > 0) wait(&mi.q_empty, (nq - 1) & 1);
+        ++nq;
+        if (lane == 0) {
+          constexpr int TILES = MT2 ? 2 : 1;
+          mbar_expect_tx(&mi.q_full, TILES * C::TILE);
+          for (int g = 0; g < TILES; ++g)
+            for (int bx = 0; bx < C::BOXES; ++bx)
+              tma_load_4d(sm + g * C::TILE + bx * 128 * 128, &p.tmQ, 0, pc.kvh * G,
+                          pc.s.row0 + (pc.m0 + g * 128) / G, bx, &mi.q_full);
+        }
+      }
+      if (*reinterpret_cast<volatile int*>(&mi.failed) && nq > 0) mbar_wait(&mi.q_full, (nq - 1) & 1, &g_error, 1);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
@@ -553,41 +607,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int g = warp >> 2, r = tid & 127;          // warpgroup, row of its 128-row tile
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane of the warp's first row
     const uint32_t s_col = tmem + lanes + g * 128, o_col = tmem + lanes + 256 + g * HD;
-    int ns = 0;  // score tiles of this warpgroup so far
+    int ns = 0, nl = 0;  // score tiles of this warpgroup so far, tiles looked over
     while (next_warp()) {
       const Span& s = pc.s;
       const int m = pc.m0 + (MT2 ? g * 128 : 0) + r, t = m / G, head = pc.kvh * G + m % G;
       const bool live = t < s.T;
       const int pos = live ? row_position(p, s, t) : s.ctx;
       const bool warp_live = __any_sync(0xffffffffu, live);
-      // Q rows into shared memory: MT2, own tile; key split, half of the one tile each
-      constexpr int QN = MT2 ? 128 : 256, QI = 128 * (HD / 8) / QN;
-      uint8_t* qt = sm + (MT2 ? g * C::TILE : 0);
-      const int qm = pc.m0 + (MT2 ? g * 128 : 0), qx = MT2 ? r : tid;
-      if (p.q_f16) {
-#pragma unroll
-        for (int it = 0; it < QI; ++it) {
-          const int x = it * QN + qx, rr = x / (HD / 8), ch = x % (HD / 8), mm = qm + rr, tt = mm / G;
-          const bool ok = tt < s.T;
-          const long long at =
-              ok ? (long long)(s.row0 + tt) * p.ldq + (long long)(pc.kvh * G + mm % G) * HD + ch * 8 : 0;
-          cp_async16(qt + sw(rr, ch, 128), static_cast<const uint16_t*>(p.q) + at, ok);
-          if (X2) *reinterpret_cast<uint4*>(qt + C::TILE + sw(rr, ch, 128)) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-      } else {
+      if (!q_tma) {
+        // Q rows into shared memory: MT2, own tile; key split, half of the one tile each.  This
+        // warpgroup's (key split: both) scores of the unit before are formed.
+        constexpr int QN = MT2 ? 128 : 256;
 #pragma unroll 2
-        for (int it = 0; it < QI; ++it) {
-          const int x = it * QN + qx, rr = x / (HD / 8), ch = x % (HD / 8), mm = qm + rr, tt = mm / G;
+        for (int x = MT2 ? r : tid; x < 128 * (HD / 8); x += QN) {
+          const int rr = x / (HD / 8), ch = x % (HD / 8), mm = pc.m0 + (MT2 ? g * 128 : 0) + rr, tt = mm / G;
           uint4 h = make_uint4(0u, 0u, 0u, 0u), l = h;
-          if (tt < s.T) q_chunk(p, s.row0 + tt, pc.kvh * G + mm % G, HD, ch, h, l);
-          *reinterpret_cast<uint4*>(qt + sw(rr, ch, 128)) = h;
-          if (X2) *reinterpret_cast<uint4*>(qt + C::TILE + sw(rr, ch, 128)) = l;
+          if (tt < s.T) q_chunk(p, (long long)(s.row0 + tt) * p.ldq + (long long)(pc.kvh * G + mm % G) * HD + ch * 8, h, l);
+          uint8_t* dst = sm + (MT2 ? g * C::TILE : 0) + sw(rr, ch, 128);
+          *reinterpret_cast<uint4*>(dst) = h;
+          if (X2) *reinterpret_cast<uint4*>(dst + C::TILE) = l;
         }
+        fence_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&mi.q_full);
       }
-      fence_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&mi.q_full[MT2 ? g : 0]);
       {  // O starts at zero: every product adds to it
         uint32_t z[32];
 #pragma unroll
@@ -597,58 +640,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_st();
       }
       float ref = -INFINITY, sum = 0.f;
-      // pages of a tile that do not exist (the TMA warp skips them): lanes 0-7 look one tile ahead
-      auto page_ok = [&](int tile) {
-        const int pg = s.lo / 16 + (pc.t0 + tile) * (kKeys / 16) + lane;
-        if (lane >= kKeys / 16 || tile >= pc.nt || pg >= p.max_blocks || pg * 16 >= s.hi) return false;
-        const int id = p.block_table[(long long)pc.b * p.max_blocks + pg];
-        return id >= 0 && id < p.n_blocks;
-      };
+      auto page_ok = [&](int tile) { return page_exists(p, pc, tile, lane); };
       bool have = page_ok(MT2 ? 0 : g);
 
       for (int i = MT2 ? 0 : g; i < pc.nt; i += PER) {
         const int c = vc + i, vs = c % C::SV, j0 = s.lo + (pc.t0 + i) * kKeys;
         const unsigned miss = ~__ballot_sync(0xffffffffu, have) & 0xffu;
         have = page_ok(i + PER);
-        const bool whole = miss == 0 && j0 + kKeys <= s.ctx && (p.window == 0 || j0 > s.pmax - p.window);
+        const bool whole = whole_tile(p, s, j0, miss);
         // the scores being there, this warpgroup's last product is done: its V stage has turned over,
         // and a wait for the next tile in it cannot mistake the phase
         wait(&mi.s_full[g], ns & 1);
         ++ns;
         fence_after();
-        unsigned bad[4] = {0u, 0u, 0u, 0u};
-        if (!whole) {
-          // zero the V rows past the end or without a page, find and zero non-finite ones; MT2
-          // shares the tile, and the two warpgroups do half each
-          wait(&mi.v_full[vs], (c / C::SV) & 1);
-          uint8_t* V = sm + C::OFF_V + vs * C::TILE;
-          const int id = MT2 ? 3 : 1 + g, n = MT2 ? 256 : 128, me = MT2 ? tid : r;
-          unsigned* flags = mi.bad[MT2 ? 0 : g];
-          for (int x = me; x < kKeys * (HD / 8); x += n) {
-            const int rr = x / (HD / 8), ch = x % (HD / 8);
-            uint4* v = reinterpret_cast<uint4*>(V + v_at<HD>(rr, ch));
-            if (j0 + rr >= s.hi || ((miss >> (rr >> 4)) & 1)) {
-              *v = make_uint4(0u, 0u, 0u, 0u);
-            } else if (nonfinite(*v)) {
-              atomicOr(&flags[rr >> 5], 1u << (rr & 31));
-            }
-          }
-          fence_async();
-          bar_sync(id, n);
-#pragma unroll
-          for (int w = 0; w < 4; ++w) bad[w] = *reinterpret_cast<volatile unsigned*>(&flags[w]);
-          if (bad[0] | bad[1] | bad[2] | bad[3]) {
-            for (int x = me; x < kKeys * (HD / 8); x += n) {
-              const int rr = x / (HD / 8), ch = x % (HD / 8);
-              if ((bad[rr >> 5] >> (rr & 31)) & 1)
-                *reinterpret_cast<uint4*>(V + v_at<HD>(rr, ch)) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            fence_async();
-            bar_sync(id, n);
-            if (me < 4) flags[me] = 0u;
-            bar_sync(id, n);
-          }
-        }
         if (warp_live) {
           unsigned see[4];  // formed before the scores fill the registers
           if (!whole) {
@@ -738,21 +742,52 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const float2 s01 = split(add2(acc[0], acc[1]));
           sum += s01.x + s01.y;
-          if (bad[0] | bad[1] | bad[2] | bad[3]) {  // non-finite V rows: the rows that see them alone
-            tmem_wait_st();
-#pragma unroll 1
-            for (int k = 0; k < kKeys; ++k) {
-              if (!((bad[k >> 5] >> (k & 31)) & 1u)) continue;
-              const float2 w2 = h2f2(tmem_ld1(s_col + k / 2));
-              float w = (k & 1) ? w2.y : w2.x;
-              if constexpr (X2) {
-                const float2 l2 = h2f2(tmem_ld1(s_col + 64 + k / 2));
-                w += (k & 1) ? l2.y : l2.x;
-              }
-              add_place<HD>(p, pc.b, pc.kvh, j0 + k, w, o_col);
-            }
-          }
           tmem_wait_st();
+        }
+        if (!whole) {
+          // V rows past the end or without a page become zero and non-finite ones are found, by the
+          // warps that share the tile (MT2: all eight); each of them hears of it through v_seen
+          const int id = MT2 ? 0 : g, n = MT2 ? 256 : 128;
+          unsigned* bad = mi.bad[id][nl % 3];
+          wait(&mi.v_full[vs], (c / C::SV) & 1);
+          uint8_t* V = sm + C::OFF_V + vs * C::TILE;
+#pragma unroll 4
+          for (int x = MT2 ? tid : r; x < kKeys * (HD / 8); x += n) {
+            const int rr = x / (HD / 8), ch = x % (HD / 8);
+            uint4* v = reinterpret_cast<uint4*>(V + v_at<HD>(rr, ch));
+            const uint4 u = *v;
+            if (j0 + rr >= s.hi || ((miss >> (rr >> 4)) & 1)) *v = make_uint4(0u, 0u, 0u, 0u);
+            else if (nonfinite(u)) atomicOr(&bad[rr >> 5], 1u << (rr & 31));
+          }
+          // the flags of the next such tile: everyone is past the tile that used them last
+          if ((MT2 ? tid : r) < 4) mi.bad[id][(nl + 1) % 3][tid & 3] = 0u;
+          fence_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&mi.v_seen[id]);
+          wait(&mi.v_seen[id], nl & 1);
+          ++nl;
+          if (bad[0] | bad[1] | bad[2] | bad[3]) {
+            // the whole rows go (each warpgroup does it before its own product), and their products
+            // are formed for the rows that see them alone
+            for (int x = r; x < kKeys * (HD / 8); x += 128) {
+              const int rr = x / (HD / 8), ch = x % (HD / 8);
+              if ((bad[rr >> 5] >> (rr & 31)) & 1)
+                *reinterpret_cast<uint4*>(V + v_at<HD>(rr, ch)) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_async();
+            if (warp_live)
+#pragma unroll 1
+              for (int k = 0; k < kKeys; ++k) {
+                if (!((bad[k >> 5] >> (k & 31)) & 1u)) continue;
+                const float2 w2 = h2f2(tmem_ld1(s_col + k / 2));
+                float w = (k & 1) ? w2.y : w2.x;
+                if constexpr (X2) {
+                  const float2 l2 = h2f2(tmem_ld1(s_col + 64 + k / 2));
+                  w += (k & 1) ? l2.y : l2.x;
+                }
+                add_place<HD>(p, pc.b, pc.kvh, j0 + k, w, o_col);
+              }
+          }
         }
         fence_before();
         __syncwarp();
