@@ -47,6 +47,11 @@ constexpr int kMaxWords = 8;
 
 __device__ int g_error;  // a bounded wait gave up (b2d_paged_tree_attn_error)
 
+// A unit of work that several CTAs share (tcgen05 kernel): CTAs blockIdx.x .. last.
+struct Split {
+  int W, last, slot, row0, T, m0, kvh;
+};
+
 struct Params {
   // page pools as [n_blocks * Hkv * 16, HD] fp16: boxes of 64 columns x 16 rows (tcgen05 kernel's V:
   // 16 rows x all 64-column blocks)
@@ -76,6 +81,7 @@ struct Params {
   int max_chunks;  // chunks per sequence
   float* part_o;   // [rows][n_heads][max_chunks][HD]
   float* part_ml;  // [rows][n_heads][max_chunks][2]
+  Split* splits;   // tcgen05 kernel: one per CTA; its part_o and part_ml are [2 * CTAs][unit rows]
 };
 
 
@@ -721,6 +727,7 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
       B2D_TRY(make_tmap_f16_heads(&p.tmQ, q, rows, n_heads, head_dim, ldq, G, 128 / G));
     p.m_tiles = h.m_tiles;
     p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + h.off_ml);
+    p.splits = reinterpret_cast<tree::Split*>(static_cast<char*>(workspace) + h.off_splits);
     if (head_dim == 64)
       return h.mt2 ? tree::t5::launch<64, true, false>(p, h, stream)
                    : (x2 ? tree::t5::launch<64, false, true>(p, h, stream)

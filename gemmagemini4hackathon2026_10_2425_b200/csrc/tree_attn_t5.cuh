@@ -165,6 +165,8 @@ struct Piece {
   int b, kvh, m0;
   int t0, nt;      // first key tile of the piece (of the unit's), number of them
   bool whole;      // the whole unit
+  bool starts;     // its first steps
+  int u_end;       // the unit's last step + 1
   int slot;        // place in the workspace, if not
 };
 
@@ -268,6 +270,8 @@ struct Walk {
     pc.t0 = s0 * PER;
     pc.nt = max(0, min(s1 * PER, tiles) - pc.t0);
     pc.whole = s0 == 0 && s1 == n;
+    pc.starts = s0 == 0;
+    pc.u_end = at0 + (pc.kvh + 1) * n;
     pc.slot = 2 * (int)blockIdx.x + (first ? 0 : 1);
     x += s1 - s0;
     first = false;
@@ -319,12 +323,18 @@ __device__ __forceinline__ void add_place(const Params& p, int b, int kvh, int j
   tmem_wait_st();
 }
 
-// Whether the page of lane 0-7 of a tile exists (the V loader skips it otherwise).
-__device__ __forceinline__ bool page_exists(const Params& p, const Piece& pc, int tile, int lane) {
+// Block-table entry of lane 0-7's page of a tile (-1: none).  Callers load it a tile ahead and
+// compare it only when they come to the tile: a comparison would wait for the load on the spot.
+__device__ __forceinline__ int page_entry(const Params& p, const Piece& pc, int tile, int lane) {
   const int pg = pc.s.lo / 16 + (pc.t0 + tile) * (kKeys / 16) + lane;
-  if (lane >= kKeys / 16 || tile >= pc.nt || pg >= p.max_blocks || pg * 16 >= pc.s.hi) return false;
-  const int id = p.block_table[(long long)pc.b * p.max_blocks + pg];
-  return id >= 0 && id < p.n_blocks;
+  int id = -1;
+  if (lane < kKeys / 16 && tile < pc.nt && pg < p.max_blocks && pg * 16 < pc.s.hi)
+    id = p.block_table[(long long)pc.b * p.max_blocks + pg];
+  return id;
+}
+// Bit per page of the tile that does not exist (the loaders skip it).
+__device__ __forceinline__ unsigned missing(const Params& p, int entry) {
+  return ~__ballot_sync(0xffffffffu, entry >= 0 && entry < p.n_blocks) & 0xffu;
 }
 // Whether every row sees every place of the tile from j0 on.
 __device__ __forceinline__ bool whole_tile(const Params& p, const Span& s, int j0, unsigned miss) {
@@ -370,6 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // fp16 rows whose heads fill a 128-row tile exactly come by TMA; others the softmax warps load
   const bool q_tma = p.q_f16 && 128 % G == 0;
 
+  pdl_launch_dependents();  // the join waits for this grid's end before it reads anything
   if (tid == 0) {
     for (int i = 0; i < C::SK; ++i) {
       mbar_init(&mi.k_full[i], 1);
@@ -436,16 +447,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint64_t* full = is_k ? mi.k_full : mi.v_full;
       uint64_t* empty = is_k ? mi.k_empty : mi.v_empty;
       while (!dead && next_warp()) {
-        const int* bt = p.block_table + (long long)pc.b * p.max_blocks;
-        const int page0 = pc.s.lo / 16 + pc.t0 * (kKeys / 16);
-        auto page_id = [&](int tile) {
-          const int pg = page0 + tile * (kKeys / 16) + lane;
-          const int id = (lane < kKeys / 16 && tile < pc.nt && pg < p.max_blocks && pg * 16 < pc.s.hi) ? bt[pg] : -1;
-          return id >= 0 && id < p.n_blocks ? id : -1;
-        };
-        int id = page_id(0);
+        int entry = page_entry(p, pc, 0, lane);
         for (int i = 0; i < pc.nt; ++i, ++kc) {
-          const int ahead = page_id(i + 1);
+          const int id = entry >= 0 && entry < p.n_blocks ? entry : -1;
+          entry = page_entry(p, pc, i + 1, lane);
           const unsigned have = __ballot_sync(0xffffffffu, id >= 0);
           const int row = (id * p.n_kv + pc.kvh) * 16, st = kc % stages;
           if (kc >= stages) wait(&empty[st], (kc / stages - 1) & 1);
@@ -466,7 +471,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               tma_load_3d(sm + C::OFF_V + st * C::TILE + lane * (HD * 32), &p.tmV, 0, row, 0, &full[st]);
             }
           }
-          id = ahead;
         }
       }
       if (*reinterpret_cast<volatile int*>(&mi.failed)) {  // copies in flight land before the CTA ends
@@ -502,10 +506,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
         };
-        bool have = page_exists(p, pc, 0, lane);
-        auto miss_at = [&](int i) {  // called for tile 0, 1, ...; looks one ahead
-          const unsigned m = ~__ballot_sync(0xffffffffu, have) & 0xffu;
-          have = page_exists(p, pc, i + 1, lane);
+        int entry = page_entry(p, pc, 0, lane);
+        auto miss_at = [&](int i) {  // called for tile 0, 1, ...
+          const unsigned m = missing(p, entry);
+          entry = page_entry(p, pc, i + 1, lane);
           return m;
         };
         auto pv = [&](int g, int i, bool first, bool last) {  // O_g += P_g V of tile i
@@ -607,6 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int g = warp >> 2, r = tid & 127;          // warpgroup, row of its 128-row tile
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane of the warp's first row
     const uint32_t s_col = tmem + lanes + g * 128, o_col = tmem + lanes + 256 + g * HD;
+    Split shared_unit = {0, -1, 0, 0, 0, 0, 0};  // thread 0: the unit that other CTAs go on with
     int ns = 0, nl = 0;  // score tiles of this warpgroup so far, tiles looked over
     while (next_warp()) {
       const Span& s = pc.s;
@@ -640,13 +645,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_st();
       }
       float ref = -INFINITY, sum = 0.f;
-      auto page_ok = [&](int tile) { return page_exists(p, pc, tile, lane); };
-      bool have = page_ok(MT2 ? 0 : g);
+      int entry = page_entry(p, pc, MT2 ? 0 : g, lane);
 
       for (int i = MT2 ? 0 : g; i < pc.nt; i += PER) {
         const int c = vc + i, vs = c % C::SV, j0 = s.lo + (pc.t0 + i) * kKeys;
-        const unsigned miss = ~__ballot_sync(0xffffffffu, have) & 0xffu;
-        have = page_ok(i + PER);
+        const unsigned miss = missing(p, entry);
+        entry = page_entry(p, pc, i + PER, lane);
         const bool whole = whole_tile(p, s, j0, miss);
         // the scores being there, this warpgroup's last product is done: its V stage has turned over,
         // and a wait for the next tile in it cannot mistake the phase
@@ -795,6 +799,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       kc += pc.nt;
       vc += pc.nt;
+      if (tid == 0 && pc.starts && !pc.whole) {
+        int last = blockIdx.x;  // the CTA with the unit's last piece
+        while (part_begin(W, last + 1, gridDim.x) < pc.u_end) ++last;
+        shared_unit = Split{W, last, pc.slot, s.row0, s.T, pc.m0, pc.kvh};
+      }
 
       // ---- the unit's (or piece's) result
       const bool any_tile = (MT2 ? 0 : g) < pc.nt;
@@ -853,6 +862,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_after();
       }
     }
+    if (tid == 0) p.splits[blockIdx.x] = shared_unit;
   }
   fence_before();
   __syncthreads();
@@ -861,61 +871,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
 }
 
-// Joins the pieces of each unit that more than one CTA worked on; one warp per row.
-template <int HD, int ROWS, int PER>
-__global__ void __launch_bounds__(256) tree_join_t5_kernel(const Params p, int ctas, int stride) {
-  __shared__ int prefix[kGroups + 1];
-  __shared__ Scan scan;
-  const int G = p.n_heads / p.n_kv;
-  const int b = blockIdx.z, mt = blockIdx.y / p.n_kv, kvh = blockIdx.y % p.n_kv;
-  Span s;
-  const int n = unit_steps<ROWS, PER>(p, b, mt, G, s);
-  if (n == 0) return;
-  steps_prefix<ROWS, PER>(p, G, stride, prefix, scan);
-  const int W = prefix[groups_of(p.batch, stride)];
-  int u0 = prefix[b / stride];
-  for (int i = b / stride * stride; i < b; ++i) u0 += sequence_steps<ROWS, PER>(p, i, G);
-  for (int i = 0; i < mt; ++i) {
-    Span q;
-    u0 += p.n_kv * unit_steps<ROWS, PER>(p, b, i, G, q);
+// Joins the pieces of each unit that more than one CTA worked on: blockIdx.x is the CTA with the
+// unit's first piece (a CTA has one such unit at most, its last), one warp per row.
+template <int HD, int ROWS>
+__global__ void __launch_bounds__(256) tree_join_t5_kernel(const Params p, int ctas) {
+  pdl_wait();
+  const Split sp = p.splits[blockIdx.x];
+  const int rr = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int G = p.n_heads / p.n_kv, t = (sp.m0 + rr) / G;
+  if (sp.last <= (int)blockIdx.x || t >= sp.T) return;
+  constexpr int E = HD / 32;
+  // the places of the unit's pieces: the CTA's last one here, the first one of the CTAs after it
+  // (those without any step hold nothing)
+  auto state = [&](int c) { return (long long)(c == (int)blockIdx.x ? sp.slot : 2 * c) * ROWS + rr; };
+  auto none = [&](int c) { return part_begin(sp.W, c, ctas) == part_begin(sp.W, c + 1, ctas); };
+  float top = -INFINITY, total = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int c = blockIdx.x; c <= sp.last; ++c) {
+    if (none(c)) continue;
+    const long long st = state(c);
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + st * 2);
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = p.part_o[st * HD + e * 32 + lane];
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;  // nothing seen in this piece
+    const float m = fmaxf(top, ml.x), base = m == -INFINITY ? 0.f : m;
+    const float w0 = ex2(top - base), w1 = ex2(ml.x - base);
+    top = m;
+    total = total * w0 + ml.y * w1;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = acc[e] * w0 + v[e] * w1;
   }
-  u0 += kvh * n;
-  // the CTAs whose parts hold the unit's first and last step
-  int c0 = (int)((long long)u0 * ctas / W);
-  while (part_begin(W, c0 + 1, ctas) <= u0) ++c0;
-  while (part_begin(W, c0, ctas) > u0) --c0;
-  int c1 = c0;
-  while (part_begin(W, c1 + 1, ctas) < u0 + n) ++c1;
-  if (c1 == c0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int rr = blockIdx.x * 8 + warp; rr < ROWS; rr += gridDim.x * 8) {
-    const int m = mt * ROWS + rr, t = m / G;
-    if (t >= s.T) break;
-    // a CTA's place for this unit: its first piece begins with the CTA's part
-    auto state = [&](int c) { return (long long)(2 * c + (part_begin(W, c, ctas) < u0 ? 1 : 0)) * ROWS + rr; };
-    auto empty = [&](int c) { return part_begin(W, c, ctas) == part_begin(W, c + 1, ctas); };
-    float top = -INFINITY;
-    for (int c = c0; c <= c1; ++c)
-      if (!empty(c)) top = fmaxf(top, p.part_ml[state(c) * 2]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float total = 0.f, acc[HD / 32];
+  const float inv = total == 0.f ? 0.f : 1.0f / total;
+  const long long at = (long long)(sp.row0 + t) * p.ldout + (long long)(sp.kvh * G + (sp.m0 + rr) % G) * HD;
 #pragma unroll
-    for (int e = 0; e < HD / 32; ++e) acc[e] = 0.f;
-    for (int c = c0; c <= c1; ++c) {
-      if (empty(c)) continue;  // fewer steps than CTAs
-      const long long st = state(c);
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + st * 2);
-      const float w = ex2(ml.x - base);
-      if (ml.x == -INFINITY && ml.y == 0.f) continue;  // nothing seen in this piece
-      total = fmaf(w, ml.y, total);
-#pragma unroll
-      for (int e = 0; e < HD / 32; ++e) acc[e] = fmaf(w, p.part_o[st * HD + e * 32 + lane], acc[e]);
-    }
-    const float inv = total == 0.f ? 0.f : 1.0f / total;
-    const long long at = (long long)(s.row0 + t) * p.ldout + (long long)(kvh * G + m % G) * HD;
-#pragma unroll
-    for (int e = 0; e < HD / 32; ++e) store_out(p, at + e * 32 + lane, acc[e] * inv);
-  }
+  for (int e = 0; e < E; ++e) store_out(p, at + e * 32 + lane, acc[e] * inv);
 }
 
 // Whether this kernel serves the call (the other one has no limits of this kind).
@@ -929,7 +920,7 @@ struct Shape {
   bool mt2;
   int rows, m_tiles, grid, stride;
   long long max_steps;
-  size_t off_ml, bytes;
+  size_t off_ml, off_splits, bytes;
 };
 static Shape shape_of(int batch, int n_heads, int n_kv, int head_dim, int max_q, int max_ctx, bool x2) {
   Shape h;
@@ -943,7 +934,8 @@ static Shape shape_of(int batch, int n_heads, int n_kv, int head_dim, int max_q,
   h.stride = (batch + kGroups - 1) / kGroups;
   h.grid = (int)std::min<long long>(num_sms(), h.max_steps);
   h.off_ml = (size_t)2 * h.grid * h.rows * head_dim * sizeof(float);
-  h.bytes = h.off_ml + (size_t)2 * h.grid * h.rows * 2 * sizeof(float);
+  h.off_splits = h.off_ml + (size_t)2 * h.grid * h.rows * 2 * sizeof(float);
+  h.bytes = h.off_splits + h.grid * sizeof(Split);
   return h;
 }
 
@@ -961,9 +953,7 @@ static int launch(Params& p, const Shape& h, cudaStream_t stream) {
   }
   kern<<<h.grid, kThreads, smem, stream>>>(p, h.stride);
   B2D_TRY(launch_status());
-  tree_join_t5_kernel<HD, C::ROWS, MT2 ? 1 : 2>
-      <<<dim3(C::ROWS / 32, h.m_tiles * p.n_kv, p.batch), 256, 0, stream>>>(p, h.grid, h.stride);
-  return launch_status();
+  return launch_pdl(tree_join_t5_kernel<HD, C::ROWS>, dim3(h.grid, C::ROWS / 8), dim3(256), 0, stream, p, h.grid);
 }
 
 }  // namespace t5
