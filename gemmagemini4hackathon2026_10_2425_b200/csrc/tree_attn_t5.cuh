@@ -323,24 +323,23 @@ __device__ __forceinline__ void add_place(const Params& p, int b, int kvh, int j
   tmem_wait_st();
 }
 
-// Block-table entry of lane 0-7's page of a tile (-1: none).  Callers load it a tile ahead and
-// compare it only when they come to the tile: a comparison would wait for the load on the spot.
-__device__ __forceinline__ int page_entry(const Params& p, const Piece& pc, int tile, int lane) {
-  const int pg = pc.s.lo / 16 + (pc.t0 + tile) * (kKeys / 16) + lane;
-  int id = -1;
-  if (lane < kKeys / 16 && tile < pc.nt && pg < p.max_blocks && pg * 16 < pc.s.hi)
-    id = p.block_table[(long long)pc.b * p.max_blocks + pg];
-  return id;
-}
+// The block-table entries of a piece's tiles, lane 0-7 a page each (-1: none).  Callers load an
+// entry a tile ahead and compare it only when they come to the tile: a comparison would wait for
+// the load on the spot.
+struct Pages {
+  const int* at;  // the lane's entry of tile 0
+  int left;       // entries of the lane's column, from tile 0 on, that hold a page (in pages)
+  __device__ Pages(const Params& p, const Piece& pc, int lane) {
+    const int pg = pc.s.lo / 16 + pc.t0 * (kKeys / 16) + lane;
+    at = p.block_table + (long long)pc.b * p.max_blocks + pg;
+    left = lane < kKeys / 16 ? min(min(p.max_blocks, (pc.s.hi + 15) / 16), pg - lane + pc.nt * (kKeys / 16)) - pg : 0;
+  }
+  __device__ int operator()(int tile) const { return tile * (kKeys / 16) < left ? at[tile * (kKeys / 16)] : -1; }
+};
 // Bit per page of the tile that does not exist (the loaders skip it).
 __device__ __forceinline__ unsigned missing(const Params& p, int entry) {
   return ~__ballot_sync(0xffffffffu, entry >= 0 && entry < p.n_blocks) & 0xffu;
 }
-// Whether every row sees every place of the tile from j0 on.
-__device__ __forceinline__ bool whole_tile(const Params& p, const Span& s, int j0, unsigned miss) {
-  return miss == 0 && j0 + kKeys <= s.ctx && (p.window == 0 || j0 > s.pmax - p.window);
-}
-
 // Bits of the places k0 .. k0 + 31 that row t (of the sequence's own rows, at position pos) sees,
 // but for pages that do not exist.
 __device__ __forceinline__ unsigned range_bits(int k0, int lo, int hi) {  // places [lo, hi)
@@ -447,12 +446,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint64_t* full = is_k ? mi.k_full : mi.v_full;
       uint64_t* empty = is_k ? mi.k_empty : mi.v_empty;
       while (!dead && next_warp()) {
-        int entry = page_entry(p, pc, 0, lane);
-        for (int i = 0; i < pc.nt; ++i, ++kc) {
+        const Pages pages(p, pc, lane);
+        const int nt = pc.nt, kvh = pc.kvh;
+        int entry = pages(0);
+        for (int i = 0; i < nt; ++i, ++kc) {
           const int id = entry >= 0 && entry < p.n_blocks ? entry : -1;
-          entry = page_entry(p, pc, i + 1, lane);
+          entry = pages(i + 1);
           const unsigned have = __ballot_sync(0xffffffffu, id >= 0);
-          const int row = (id * p.n_kv + pc.kvh) * 16, st = kc % stages;
+          const int row = (id * p.n_kv + kvh) * 16, st = kc % stages;
           if (kc >= stages) wait(&empty[st], (kc / stages - 1) & 1);
           dead = __any_sync(0xffffffffu, dead);
           if (dead) break;
@@ -484,7 +485,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       // time: 275 us instead of TODO for 8 trees of 64 nodes over 8k-32k places.)
       const uint32_t sm0 = smem_u32(sm);
       int np[2] = {0, 0}, nq = 0;  // products issued per warpgroup, pieces begun
-      int ns[2] = {0, 0};          // tiles looked over per warpgroup (MT2: ns[0])
       while (next_warp()) {
         auto qk = [&](int g, int i, bool first, bool last) {  // S_g = Q_g K^T of tile i of the piece
           const int c = kc + i, ks = c % C::SK;
@@ -506,18 +506,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
         };
-        int entry = page_entry(p, pc, 0, lane);
-        auto miss_at = [&](int i) {  // called for tile 0, 1, ...
-          const unsigned m = missing(p, entry);
-          entry = page_entry(p, pc, i + 1, lane);
-          return m;
-        };
         auto pv = [&](int g, int i, bool first, bool last) {  // O_g += P_g V of tile i
           const int c = vc + i, vs = c % C::SV;
-          if (first) {
-            wait(&mi.v_full[vs], (c / C::SV) & 1);
-            if (!whole_tile(p, pc.s, pc.s.lo + (pc.t0 + i) * kKeys, miss_at(i))) wait(&mi.v_seen[MT2 ? 0 : g], ns[g]++ & 1);
-          }
+          // (a tile that some row must not see all of has been looked over before its weights are
+          // announced: no wait of its own for that)
+          if (first) wait(&mi.v_full[vs], (c / C::SV) & 1);
           wait(&mi.p_full[g], np[g] & 1);
           fence_after();
           const uint32_t v = desc_mn(sm0 + C::OFF_V + vs * C::TILE, 2048);
@@ -645,13 +638,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_st();
       }
       float ref = -INFINITY, sum = 0.f;
-      int entry = page_entry(p, pc, MT2 ? 0 : g, lane);
+      const Pages pages(p, pc, lane);
+      const int nt = pc.nt, first_j = s.lo + pc.t0 * kKeys;
+      // tiles before this place are seen whole by every row, unless a page is missing or the window cuts
+      const int whole_end = s.ctx - kKeys, whole_begin = p.window == 0 ? INT_MIN : s.pmax - p.window + 1;
+      int entry = pages(MT2 ? 0 : g);
 
-      for (int i = MT2 ? 0 : g; i < pc.nt; i += PER) {
-        const int c = vc + i, vs = c % C::SV, j0 = s.lo + (pc.t0 + i) * kKeys;
+      for (int i = MT2 ? 0 : g; i < nt; i += PER) {
+        const int c = vc + i, vs = c % C::SV, j0 = first_j + i * kKeys;
         const unsigned miss = missing(p, entry);
-        entry = page_entry(p, pc, i + PER, lane);
-        const bool whole = whole_tile(p, s, j0, miss);
+        entry = pages(i + PER);
+        const bool whole = miss == 0 && j0 <= whole_end && j0 >= whole_begin;
         // the scores being there, this warpgroup's last product is done: its V stage has turned over,
         // and a wait for the next tile in it cannot mistake the phase
         wait(&mi.s_full[g], ns & 1);
