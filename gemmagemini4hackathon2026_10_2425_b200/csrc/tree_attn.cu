@@ -89,6 +89,7 @@ struct Params {
 struct Span {
   int row0, T, ctx;  // first row, rows, cached places
   int lo, hi;        // places [lo, hi) that any of the tile's rows may see; lo a multiple of `keys`
+  int all;           // every row sees the places before this one (but for the window)
   int pmax;          // no row's position is larger
   __device__ int chunks(int chunk) const { return hi > lo ? (hi - lo + chunk - 1) / chunk : 0; }
 };
@@ -100,6 +101,7 @@ __device__ __forceinline__ bool span_of(const Params& p, int b, int m0, int m1, 
   if (s.row0 < 0 || s.T <= 0 || s.ctx < 0 || s.ctx > p.max_ctx - s.T) return false;
   const int t0 = m0 / G, t1 = min((m1 - 1) / G, s.T - 1);  // the tile's rows
   if (t0 >= s.T) return false;
+  s.all = p.mask ? s.ctx : s.ctx + t0 + 1;
   s.pmax = s.ctx + t1;
   s.hi = p.mask ? s.ctx + s.T : s.ctx + t1 + 1;
   // row t's position is at least ctx (a tree) or ctx + t
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
       uint8_t* Kt = ring + st * 2 * C::TILE;
       uint8_t* Vt = Kt + C::TILE;
       // does every row of the tile see every key of it?
-      bool whole = j0 + kKeys <= s.ctx && (p.window == 0 || j0 > s.pmax - p.window);
+      bool whole = j0 + kKeys <= s.all && (p.window == 0 || j0 > s.pmax - p.window);
 #pragma unroll
       for (int pg = 0; pg < kKeys / 16; ++pg) whole &= blk[i * (kKeys / 16) + pg] >= 0;
       unsigned long long bad = 0ull;

@@ -170,6 +170,13 @@ struct Piece {
   int slot;        // place in the workspace, if not
 };
 
+// What beginning and ending a unit costs, in steps: the line counts it in, or the CTAs with many short
+// units would end last (4 x 512 causal rows over 0-8k places: TODO).
+template <int PER>
+constexpr __host__ __device__ int unit_cost() {
+  return PER == 1 ? 3 : 2;
+}
+
 // Steps of one unit of sequence b, row tile mt.
 template <int ROWS, int PER>
 __device__ __forceinline__ int unit_steps(const Params& p, int b, int mt, int G, Span& s) {
@@ -177,7 +184,7 @@ __device__ __forceinline__ int unit_steps(const Params& p, int b, int mt, int G,
   return max(1, (s.hi - s.lo + kKeys * PER - 1) / (kKeys * PER));
 }
 
-// Steps of sequence b.
+// Steps of sequence b, with its units' cost.
 template <int ROWS, int PER>
 __device__ int sequence_steps(const Params& p, int b, int G) {
   int n = 0;
@@ -185,12 +192,12 @@ __device__ int sequence_steps(const Params& p, int b, int G) {
   for (int mt = 0; mt < p.m_tiles; ++mt) {
     const int u = unit_steps<ROWS, PER>(p, b, mt, G, s);
     if (u == 0) break;
-    n += u;
+    n += u + unit_cost<PER>();
   }
   return n * p.n_kv;
 }
 
-// prefix[j] = steps of the sequences before j * stride; all threads of the CTA.
+// prefix[j] = steps (with the units' cost) of the sequences before j * stride; all threads of the CTA.
 struct Scan {
   int carry, wsum[32];
 };
@@ -234,11 +241,10 @@ template <int ROWS, int PER>
 struct Walk {
   int x, end;
   int b, mt, n, at0;  // the units of row tile mt of sequence b, n steps each, begin at step at0
-  bool first;
+  int begun;          // where the CTA's part begins
   __device__ void begin(const Params& p, const int* prefix, int stride, int W) {
-    x = part_begin(W, blockIdx.x, gridDim.x);
+    x = begun = part_begin(W, blockIdx.x, gridDim.x);
     end = part_begin(W, blockIdx.x + 1, gridDim.x);
-    first = true;
     int lo = 0, hi = groups_of(p.batch, stride);  // the group of sequences that holds step x
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -250,32 +256,38 @@ struct Walk {
     n = 0;
     at0 = prefix[lo];
   }
+  // A unit's place in the line is its cost, then its steps; a part that holds the cost alone holds
+  // none of the unit.
   __device__ bool next(const Params& p, int G, Piece& pc) {
-    if (x >= end) return false;
-    Span s = pc.s;
-    while (x >= at0 + n * p.n_kv) {  // on to the units of the next row tile, or sequence
-      at0 += n * p.n_kv;
-      n = ++mt < p.m_tiles ? unit_steps<ROWS, PER>(p, b, mt, G, s) : 0;
-      if (n == 0) {
-        mt = 0;
-        n = unit_steps<ROWS, PER>(p, ++b, 0, G, s);
+    constexpr int cost = unit_cost<PER>();
+    while (x < end) {
+      Span s = pc.s;
+      while (n == 0 || x >= at0 + (n + cost) * p.n_kv) {  // on to the next row tile, or sequence
+        if (n) at0 += (n + cost) * p.n_kv;
+        n = ++mt < p.m_tiles ? unit_steps<ROWS, PER>(p, b, mt, G, s) : 0;
+        if (n == 0) {
+          mt = 0;
+          n = unit_steps<ROWS, PER>(p, ++b, 0, G, s);
+        }
+        pc.s = s;
       }
+      const int kvh = (x - at0) / (n + cost), u = at0 + kvh * (n + cost);
+      const int v1 = min(u + n + cost, end), s0 = max(0, x - u - cost), s1 = max(0, v1 - u - cost);
+      pc.slot = 2 * (int)blockIdx.x + (x == begun ? 0 : 1);
+      x = v1;
+      if (s1 == s0) continue;
+      const int tiles = (pc.s.hi - pc.s.lo + kKeys - 1) / kKeys;
+      pc.b = b;
+      pc.m0 = mt * ROWS;
+      pc.kvh = kvh;
+      pc.t0 = s0 * PER;
+      pc.nt = max(0, min(s1 * PER, tiles) - pc.t0);
+      pc.whole = s0 == 0 && s1 == n;
+      pc.starts = s0 == 0;
+      pc.u_end = u + n + cost;
+      return true;
     }
-    pc.s = s;
-    pc.b = b;
-    pc.m0 = mt * ROWS;
-    pc.kvh = (x - at0) / n;
-    const int s0 = x - at0 - pc.kvh * n, s1 = min(n, s0 + (end - x));
-    const int tiles = (s.hi - s.lo + kKeys - 1) / kKeys;
-    pc.t0 = s0 * PER;
-    pc.nt = max(0, min(s1 * PER, tiles) - pc.t0);
-    pc.whole = s0 == 0 && s1 == n;
-    pc.starts = s0 == 0;
-    pc.u_end = at0 + (pc.kvh + 1) * n;
-    pc.slot = 2 * (int)blockIdx.x + (first ? 0 : 1);
-    x += s1 - s0;
-    first = false;
-    return true;
+    return false;
   }
 };
 
@@ -641,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Pages pages(p, pc, lane);
       const int nt = pc.nt, first_j = s.lo + pc.t0 * kKeys;
       // tiles before this place are seen whole by every row, unless a page is missing or the window cuts
-      const int whole_end = s.ctx - kKeys, whole_begin = p.window == 0 ? INT_MIN : s.pmax - p.window + 1;
+      const int whole_end = s.all - kKeys, whole_begin = p.window == 0 ? INT_MIN : s.pmax - p.window + 1;
       int entry = pages(MT2 ? 0 : g);
 
       for (int i = MT2 ? 0 : g; i < nt; i += PER) {
@@ -927,7 +939,7 @@ static Shape shape_of(int batch, int n_heads, int n_kv, int head_dim, int max_q,
   h.m_tiles = (int)((m + h.rows - 1) / h.rows);
   const int keys = h.mt2 ? kKeys : 2 * kKeys;
   // + 1: with a window, a unit's first tile may begin anywhere
-  h.max_steps = (long long)batch * n_kv * h.m_tiles * ((max_ctx + keys - 1) / keys + 1);
+  h.max_steps = (long long)batch * n_kv * h.m_tiles * ((max_ctx + keys - 1) / keys + 1 + (h.mt2 ? unit_cost<1>() : unit_cost<2>()));
   h.stride = (batch + kGroups - 1) / kGroups;
   h.grid = (int)std::min<long long>(num_sms(), h.max_steps);
   h.off_ml = (size_t)2 * h.grid * h.rows * head_dim * sizeof(float);
