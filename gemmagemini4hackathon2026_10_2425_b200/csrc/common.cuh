@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/b200dec.h"
 
 namespace b2d {
@@ -129,6 +131,25 @@ __device__ __forceinline__ float gelu_tanh(float x) {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;");
+}
+
+// Allow `kern` up to `bytes` of dynamic shared memory on the current device; asked of the runtime
+// once per device (`done` is the kernel's own bit set, one bit per device).
+template <class Kern>
+inline int allow_smem(Kern kern, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+  if (e == cudaSuccess && !(done.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  }
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    cudaGetLastError();
+    return B2D_ERR_CUDA;
+  }
+  return B2D_OK;
 }
 
 // Launch with programmatic dependent launch allowed (the kernel must call pdl_wait() before it

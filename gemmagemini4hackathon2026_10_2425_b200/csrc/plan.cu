@@ -309,8 +309,10 @@ int paged_plan(const int* ctx_lens, const int* q_lens, const int* parents, int* 
                           n_free_out};
   const size_t smem = (size_t)(batch + 1) * sizeof(plan::Req);
   auto kern = parents ? plan::paged_plan_kernel<true> : plan::paged_plan_kernel<false>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e == cudaSuccess) {
+  static std::atomic<unsigned long long> done[2];
+  B2D_TRY(allow_smem(kern, (plan::kMaxBatch + 1) * (int)sizeof(plan::Req), done[parents != nullptr]));
+  cudaError_t e;
+  {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(8);
     cfg.blockDim = dim3(plan::kThreads);

@@ -629,12 +629,8 @@ template <int HD, bool X2>
 static int launch(const Params& p, int m_tiles, int batch, cudaStream_t stream) {
   auto kern = paged_tree_attn_kernel<HD, X2>;
   const int smem = Cfg<HD>::SMEM(X2);
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) {
-    set_cuda_error(e);
-    cudaGetLastError();
-    return B2D_ERR_CUDA;
-  }
+  static std::atomic<unsigned long long> done;
+  B2D_TRY(allow_smem(kern, smem, done));
   kern<<<dim3(p.max_chunks, m_tiles * p.n_kv, batch), kThreads, smem, stream>>>(p);
   B2D_TRY(launch_status());
   if (p.max_chunks > 1) {
@@ -679,6 +675,8 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
       max_blocks <= 0 || (long long)max_blocks * 16 < max_ctx || window < 0)
     return B2D_ERR_SHAPE;
   if (mask ? (mask_words <= 0 || mask_words > tree::kMaxWords) : mask_words != 0) return B2D_ERR_SHAPE;
+  const uint64_t prows = (uint64_t)n_blocks * n_kv_heads * 16;  // TMA coordinates are 32 bits
+  if (prows > 0x7fffffffull) return B2D_ERR_SHAPE;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return B2D_ERR_UNSUPPORTED;
   if (q_dtype != B2D_F32 && q_dtype != B2D_F16) return B2D_ERR_UNSUPPORTED;
   if (out_dtype != B2D_F32 && out_dtype != B2D_F16 && out_dtype != B2D_F16X2) return B2D_ERR_UNSUPPORTED;
@@ -691,8 +689,6 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
   if (need && (!workspace || workspace_bytes < need)) return B2D_ERR_WORKSPACE;
   if (!aligned16(workspace)) return B2D_ERR_ALIGN;
   tree::Params p = {};
-  const uint64_t prows = (uint64_t)n_blocks * n_kv_heads * 16;
-  if (prows > 0x7fffffffull) return B2D_ERR_SHAPE;
   B2D_TRY(make_tmap_f16(&p.tmK, k_pages, prows, head_dim, head_dim, 16));
   p.q = q;
   p.q_f16 = q_dtype == B2D_F16;

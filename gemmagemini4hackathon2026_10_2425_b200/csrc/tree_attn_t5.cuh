@@ -954,12 +954,8 @@ static int launch(Params& p, const Shape& h, cudaStream_t stream) {
   auto kern = tree_attn_t5_kernel<HD, MT2, X2>;
   const int smem = C::OFF_MISC + (int)sizeof(Misc<C::ROWS, MT2 ? 1 : 2>);
   static_assert(C::OFF_MISC + sizeof(Misc<C::ROWS, MT2 ? 1 : 2>) <= 227 * 1024, "shared memory of one CTA");
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) {
-    set_cuda_error(e);
-    cudaGetLastError();
-    return B2D_ERR_CUDA;
-  }
+  static std::atomic<unsigned long long> done;
+  B2D_TRY(allow_smem(kern, smem, done));
   kern<<<h.grid, kThreads, smem, stream>>>(p, h.stride);
   B2D_TRY(launch_status());
   return launch_pdl(tree_join_t5_kernel<HD, C::ROWS>, dim3(h.grid, C::ROWS / 8), dim3(256), 0, stream, p, h.grid);
