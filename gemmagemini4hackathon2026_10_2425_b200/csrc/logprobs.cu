@@ -10,12 +10,14 @@
 // is a relative error of the results.
 //
 // Top k without a second pass over the row: every thread remembers its own largest value and the
-// vector it came from (one compare per vector of the main loop).  The k-th largest of those
-// thread maxima bounds the k-th largest element from below, so all of the top k lie in the few
-// threads (about k of them) whose maximum reaches the bound: only their vectors are read again,
-// from L2, and the elements that reach the bound are ranked exactly.  Keys are (value, index)
-// pairs in one 64-bit number that are never equal, so ties go to the lowest index, and equal
-// values everywhere (an untrained model, a row of -inf) do not swamp the candidates.
+// vector it came from (one compare per vector of the main loop).  The k-th largest of the maxima
+// of 64 groups of threads bounds the k-th largest element from below, so all of the top k lie in
+// the few threads (about 64 ln(64 / (64 - k)) of them) whose maximum reaches the bound: only their
+// vectors are read again, from L2, and the elements that reach the bound are ranked exactly.
+// Keys are (value, index) pairs in one 64-bit number that are never equal, so ties go to the
+// lowest index, and equal values everywhere (an untrained model, a row of -inf) do not swamp the
+// candidates.  (Sorting all thread maxima for the tightest bound cost more than it saved: 9 us of
+// a CTA's time were spent after the main loop.)
 //
 // What bounds it: memory (one read of the logits).
 #include <cooperative_groups.h>
@@ -29,7 +31,8 @@ namespace lp {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxK = 32;
-constexpr int kBatch = 4;  // vectors in flight per thread
+constexpr int kBatch = 2;  // vectors in flight per thread (four CTAs per SM)
+constexpr int kGroup = kThreads / 64;  // threads per group of the bound
 constexpr int kCand = 1024;  // candidates ranked at once; more of them take the slow way
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr double kLn2 = 0.693147180559945309417;
@@ -69,6 +72,11 @@ __device__ __forceinline__ unsigned long long key_of(float v, unsigned idx) {
   uint32_t b = __float_as_uint(v);
   b = v != v ? 1u : ((b & 0x80000000u) ? ~b : (b | 0x80000000u));
   return ((unsigned long long)b << 32) | (uint32_t)~idx;
+}
+
+__device__ __forceinline__ float key_value(unsigned long long key) {
+  const uint32_t b = (uint32_t)(key >> 32);
+  return b == 1u ? __uint_as_float(0x7fffffffu) : __uint_as_float((b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
 }
 
 template <bool F16>
@@ -150,42 +158,17 @@ __device__ __forceinline__ Stat warp_join(Stat a) {
   return a;
 }
 
+// How many of the warp's keys (the lane's: `other`, number `j`) come before `key`, number `c`.
+__device__ __forceinline__ int rank_of(unsigned long long key, int c, unsigned long long other, int j) {
+  return __popc(__ballot_sync(0xffffffffu, other > key || (other == key && j < c)));
+}
+
 // This CTA runs / every CTA of the cluster runs (their shared memory may be written).
 __device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-}
-
-// Descending bitonic sort of one 64-bit key per lane.
-__device__ __forceinline__ unsigned long long shfl_xor64(unsigned long long v, int o) {
-  return __shfl_xor_sync(0xffffffffu, v, o);
-}
-__device__ __forceinline__ unsigned long long warp_sort(unsigned long long v) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-    for (int o = size >> 1; o > 0; o >>= 1) {
-      const unsigned long long w = shfl_xor64(v, o);
-      const bool up = (lane & size) != 0 && size < 32;  // ascending half of this stage
-      const bool low = (lane & o) == 0;
-      v = ((v > w) == (low != up)) ? v : w;
-    }
-  return v;
-}
-// Both descending: the 32 largest of the 64, descending.
-__device__ __forceinline__ unsigned long long warp_merge(unsigned long long a, unsigned long long b) {
-  const int lane = threadIdx.x & 31;
-  const unsigned long long r = __shfl_sync(0xffffffffu, b, 31 - lane);
-  unsigned long long v = a > r ? a : r;  // bitonic
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long w = shfl_xor64(v, o);
-    v = ((v > w) == ((lane & o) == 0)) ? v : w;
-  }
-  return v;
 }
 
 // Largest value of the CTA's threads, NaN if any is.
@@ -200,7 +183,7 @@ __device__ __forceinline__ float block_max_nan(float v, float* sm) {
 }
 
 template <bool F16>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Params p) {
   constexpr int VEC = Row<F16>::VEC;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
@@ -208,7 +191,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Params p
   const int row = blockIdx.x / ranks;
   if (p.n_rows && row >= *p.n_rows) return;  // the whole cluster: outputs left as they are
   __shared__ Stat w_stat[kWarps];
-  __shared__ unsigned long long w_keys[kWarps][32];
+  __shared__ unsigned long long g_tau, g_keys[64];  // largest key of each group of threads
   __shared__ unsigned long long cand[kCand];
   __shared__ unsigned short owners[kThreads];
   __shared__ float w_f[kWarps];
@@ -216,7 +199,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Params p
   __shared__ unsigned long long best;
   // rank 0's copies of every rank's results
   __shared__ Stat r_stat[8];
-  __shared__ unsigned long long r_keys[8][kMaxK];
+  __shared__ unsigned long long r_keys[8 * kMaxK];  // k per rank
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   cluster_arrive();
   const Row<F16> r(p, row);
@@ -274,18 +257,24 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Params p
     // (value, last index of its vector): not above the key of the element it stands for
     const unsigned long long mine =
         mv < 0 ? 0ull : key_of(mx, (unsigned)(r.first(mv) + VEC - 1));
-    unsigned long long s = warp_sort(mine);
-    w_keys[warp][lane] = s;
+    unsigned long long gk = mine;
+#pragma unroll
+    for (int o = kGroup / 2; o > 0; o >>= 1) {
+      const unsigned long long w = __shfl_xor_sync(0xffffffffu, gk, o);
+      gk = gk > w ? gk : w;
+    }
+    if (tid % kGroup == 0) g_keys[tid / kGroup] = gk;
     if (tid == 0) n_owners = n_cand = 0;
     __syncthreads();
-    for (int half = kWarps / 2; half > 0; half >>= 1) {
-      if (warp < half) {
-        s = warp_merge(s, w_keys[warp + half][lane]);
-        w_keys[warp][lane] = s;
-      }
-      __syncthreads();
-    }
-    const unsigned long long tau = w_keys[0][p.k - 1];
+    // the k-th largest of the 64 (equal ones, all of them empty groups, in order): a key's rank is a
+    // count of ballots, a few keys per warp
+    const unsigned long long ga = g_keys[lane], gb = g_keys[lane + 32];
+#pragma unroll
+    for (int j = warp; j < 64; j += kWarps)
+      if (rank_of(g_keys[j], j, ga, lane) + rank_of(g_keys[j], j, gb, lane + 32) == p.k - 1) g_tau = g_keys[j];
+    __syncthreads();
+    const unsigned long long tau = g_tau;
+    const float tau_v = key_value(tau);
     bool odd = false;  // a NaN (or an infinite maximum): the thread maxima say nothing
     for (int w = 0; w < kWarps; ++w) odd |= w_stat[w].s != w_stat[w].s;
     // threads that may hold an element at or above tau
@@ -299,7 +288,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Params p
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const int i = r.first(v) + e;
-          if (i < 0 || i >= r.V) continue;
+          if (f[e] < tau_v || i < 0 || i >= r.V) continue;
           const unsigned long long key = key_of(f[e], (unsigned)i);
           if (key >= tau) {
             const int at = atomicAdd(&n_cand, 1);
@@ -311,13 +300,13 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Params p
     __syncthreads();
     const int n = n_cand;
     cluster_wait();  // rank 0 runs
-    unsigned long long* out = cluster.map_shared_rank(&r_keys[rank][0], 0);
+    unsigned long long* out = cluster.map_shared_rank(&r_keys[rank * p.k], 0);
     if (n <= kCand && !odd) {
-      for (int c = tid; c < n; c += kThreads) {
+      for (int c = warp; c < n; c += kWarps) {
         const unsigned long long key = cand[c];
         int above = 0;
-        for (int j = 0; j < n; ++j) above += cand[j] > key;
-        if (above < p.k) out[above] = key;
+        for (int j0 = 0; j0 < n; j0 += 32) above += rank_of(key, c, j0 + lane < n ? cand[j0 + lane] : 0ull, j0 + lane);
+        if (lane == 0 && above < p.k) out[above] = key;
       }
       for (int j = n + tid; j < p.k; j += kThreads) out[j] = 0ull;
     } else {  // many elements above the bound (rare): the next largest key, k times
@@ -394,38 +383,50 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Params p
   }
   const bool far = odd || huge;
   // log2 of the row's sum, in log2 units of x * L (of (x - base) * L in a far row)
-  const double lz = (double)t.M + log2((double)t.s);
+  __shared__ double row_lz;
+  if (tid == 0) {
+    row_lz = (double)t.M + log2((double)t.s);
+    if (p.entropy) p.entropy[row] = (float)((row_lz - (double)t.M - (double)t.u / (double)t.s) * kLn2);
+  }
+  __syncthreads();
+  const double lz = row_lz;
   auto lp_of = [&](float x) -> float {
     if (far && base == -INFINITY) return x;
     const double d = far ? (double)x - (double)base : (double)x;
     return (float)((d * (double)kLog2e - lz) * kLn2);
   };
-  if (tid == 0 && p.entropy)
-    p.entropy[row] = (float)((log2((double)t.s) - (double)t.u / (double)t.s) * kLn2);
   for (int j = tid; j < p.n_targets; j += kThreads) {
     const int id = p.targets[(long long)row * p.n_targets + j];
     p.logprobs[(long long)row * p.n_targets + j] =
         id >= 0 && id < r.V ? lp_of(r.at(id)) : (t.s == t.s ? -INFINITY : t.s);
   }
+  // the top of the ranks' tops, one entry per warp at a time (one rank's are in order already)
   const int nk = ranks * p.k;
-  for (int c = tid; c < nk; c += kThreads) {
-    const unsigned long long key = r_keys[c / p.k][c % p.k];
-    int above = 0;
-    for (int j = 0; j < nk; ++j) {
-      const unsigned long long o = r_keys[j / p.k][j % p.k];
-      above += o > key || (o == key && j < c);
+  unsigned long long mine[8];
+  if (ranks > 1)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mine[j] = j * 32 + lane < nk ? r_keys[j * 32 + lane] : 0ull;
+  for (int c = warp; c < nk; c += kWarps) {
+    const unsigned long long key = r_keys[c];
+    int above = c;
+    if (ranks > 1) {
+      above = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j * 32 < nk) above += rank_of(key, c, mine[j], j * 32 + lane);
     }
-    if (above < p.k) {
-      const int id = (int)~(uint32_t)(key & 0xffffffffull);
-      p.top_ids[(long long)row * p.k + above] = id;
-      p.top_lp[(long long)row * p.k + above] = lp_of(r.at(id));
+    if (lane == 0 && above < p.k) {
+      p.top_ids[(long long)row * p.k + above] = (int)~(uint32_t)(key & 0xffffffffull);
+      p.top_lp[(long long)row * p.k + above] = lp_of(key_value(key));
     }
   }
 }
 
 }  // namespace lp
 
-// CTAs (one cluster) per row.
+// CTAs (one cluster) per row: several while they fill half of the machine or less.  More, to even
+// out the last wave of CTAs, cost more than they gave: each pays for its own selection (2048 rows of
+// 128256 fp32 logits 216 us with two, 193 with one).
 static int logprob_ranks(int rows, int V, bool f16) {
   int c = 1;
   const int vecs = (V + (f16 ? 7 : 3)) / (f16 ? 8 : 4);

@@ -112,10 +112,11 @@ __device__ void tree_rows(const Params& p, int row0, int n, int ctx) {
       const int d2 = __shfl_sync(0xffffffffu, depth, src);
       const int p2 = __shfl_sync(0xffffffffu, par, src);
 #pragma unroll
-      for (int w = 0; w < kMaxWords; ++w) {
-        const uint32_t m2 = __shfl_sync(0xffffffffu, m[w], src);
-        if (par >= 0) m[w] |= m2;
-      }
+      for (int w = 0; w < kMaxWords; ++w)
+        if (w < p.words) {
+          const uint32_t m2 = __shfl_sync(0xffffffffu, m[w], src);
+          if (par >= 0) m[w] |= m2;
+        }
       if (par >= 0) {
         depth += d2 + 1;
         par = p2;
@@ -198,12 +199,14 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const Params p) {
   const long long back_all = (long long)(pages >> 32);
   const int top = (int)min((long long)n_free + back_all, (long long)p.stack_cap);
 
-  // ---- released pages onto the stack, one warp per ended request
-  for (int b = gwarp; b < p.batch; b += nwarps) {
+  // ---- released pages onto the stack: a warp of every CTA per ended request, so that a long
+  // request's pages are moved by all of them (40 requests of 1024 pages: 30 us with one warp each)
+  for (int b = tid >> 5; b < p.batch; b += kThreads / 32) {
     const Req r = req[b];
     if (r.have >= 0) continue;
     const int n = -1 - r.have;
-    for (int j = lane; j < n; j += 32) {
+#pragma unroll 4
+    for (int j = rank * 32 + lane; j < n; j += ranks * 32) {
       const long long at = (long long)n_free + r.off + j;
       if (at < p.stack_cap) p.stack[at] = p.table[(size_t)b * p.max_blocks + j];
     }
@@ -243,11 +246,12 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const Params p) {
     p.cu_q[p.batch] = total;
     *p.n_free_out = top - sm_given;
   }
-  for (int b = gwarp; b < p.batch; b += nwarps) {
+  for (int b = tid >> 5; b < p.batch; b += kThreads / 32) {
     const Req r = req[b];
     if (r.have < 0 || r.off == kRefused) continue;
     const int need = (r.ctx + req[b + 1].row - r.row + 15) / 16 - r.have;
-    for (int j = lane; j < need; j += 32)
+#pragma unroll 4
+    for (int j = rank * 32 + lane; j < need; j += ranks * 32)
       p.table[(size_t)b * p.max_blocks + r.have + j] = __ldcg(p.stack + top - 1 - r.off - j);
   }
 
