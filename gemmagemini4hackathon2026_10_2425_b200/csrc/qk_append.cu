@@ -24,7 +24,8 @@ namespace b2d {
 
 namespace qka {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
+constexpr int kRounds = 3;  // heads per lane in flight
 
 struct Params {
   const void* qkv;
@@ -82,7 +83,7 @@ __device__ __forceinline__ float2 turn(int pos, float f) {
 
 // XF16: qkv is fp16; QF16: q_out is fp16
 template <int HD, bool XF16, bool QF16>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_append_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 8) qk_norm_rope_append_kernel(const Params p) {
   constexpr int L = HD / 8;             // lanes per head
   constexpr int SLOTS = kThreads / L;   // heads in flight per CTA
   __shared__ __align__(16) float2 cs[HD / 2];
@@ -94,54 +95,66 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_append_kernel(const Par
   const int tid = threadIdx.x, li = tid % L, h0 = tid / L;
   const int heads = p.n_heads + 2 * p.n_kv;
   const long long x0 = (long long)row * p.ldqkv + 4 * li;
-  if (tid < HD / 2) cs[tid] = turn(pos, p.inv_freq[tid]);
-  __syncthreads();
-  const float4 ca = *reinterpret_cast<const float4*>(&cs[4 * li]);      // c0 s0 c1 s1
-  const float4 cb = *reinterpret_cast<const float4*>(&cs[4 * li + 2]);  // c2 s2 c3 s3
   const bool put = slot >= 0 && slot < p.n_slots;
-  // heads are walked in whole rounds so that every lane of a warp takes part in the shuffles
-  for (int hb = 0; hb < heads; hb += SLOTS) {
-    const int h = hb + h0;
-    const bool live = h < heads;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-    if (live) {
-      a = load4<XF16>(p.qkv, x0 + (long long)h * HD);
-      b = load4<XF16>(p.qkv, x0 + (long long)h * HD + HD / 2);
-    }
-    const bool is_q = h < p.n_heads, is_k = !is_q && h < p.n_heads + p.n_kv;
-    const float* gamma = is_q ? p.q_gamma : (is_k ? p.k_gamma : nullptr);
-    float ss = a.x * a.x + a.y * a.y + a.z * a.z + a.w * a.w + b.x * b.x + b.y * b.y + b.z * b.z +
-               b.w * b.w;
+  // heads are walked in whole rounds so that every lane of a warp takes part in the shuffles, the
+  // loads of kRounds rounds first of all (before the angles the first time)
+  for (int hb = 0; hb < heads; hb += kRounds * SLOTS) {
+    float4 va[kRounds], vb[kRounds];
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!live) continue;
-    if (gamma || (!is_q && !is_k && p.v_norm)) {
-      const float r = rsqrtf(ss * (1.0f / HD) + p.eps);
-      float4 ga = make_float4(1.f, 1.f, 1.f, 1.f), gb = ga;
-      if (gamma) {
-        ga = *reinterpret_cast<const float4*>(gamma + 4 * li);
-        gb = *reinterpret_cast<const float4*>(gamma + HD / 2 + 4 * li);
+    for (int j = 0; j < kRounds; ++j) {
+      const int h = hb + j * SLOTS + h0;
+      va[j] = vb[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (h < heads) {
+        va[j] = load4<XF16>(p.qkv, x0 + (long long)h * HD);
+        vb[j] = load4<XF16>(p.qkv, x0 + (long long)h * HD + HD / 2);
       }
-      a = make_float4(a.x * r * ga.x, a.y * r * ga.y, a.z * r * ga.z, a.w * r * ga.w);
-      b = make_float4(b.x * r * gb.x, b.y * r * gb.y, b.z * r * gb.z, b.w * r * gb.w);
     }
-    if (is_q || is_k) {
-      const float4 u = a;
-      a = make_float4(u.x * ca.x - b.x * ca.y, u.y * ca.z - b.y * ca.w, u.z * cb.x - b.z * cb.y,
-                      u.w * cb.z - b.w * cb.w);
-      b = make_float4(b.x * ca.x + u.x * ca.y, b.y * ca.z + u.y * ca.w, b.z * cb.x + u.z * cb.y,
-                      b.w * cb.z + u.w * cb.w);
+    if (hb == 0) {
+      if (tid < HD / 2) cs[tid] = turn(pos, p.inv_freq[tid]);
+      __syncthreads();
     }
-    if (is_q) {
-      const long long o = (long long)row * p.ldq + (long long)h * HD + 4 * li;
-      store4<QF16>(p.q_out, o, a);
-      store4<QF16>(p.q_out, o + HD / 2, b);
-    } else if (put) {
-      const int kvh = is_k ? h - p.n_heads : h - p.n_heads - p.n_kv;
-      uint16_t* pages = is_k ? p.k_pages : p.v_pages;
-      const long long o = ((slot / 16 * p.n_kv + kvh) * 16 + slot % 16) * HD + 4 * li;
-      *reinterpret_cast<uint2*>(pages + o) = pack4(a);
-      *reinterpret_cast<uint2*>(pages + o + HD / 2) = pack4(b);
+    const float4 ca = *reinterpret_cast<const float4*>(&cs[4 * li]);      // c0 s0 c1 s1
+    const float4 cb = *reinterpret_cast<const float4*>(&cs[4 * li + 2]);  // c2 s2 c3 s3
+#pragma unroll
+    for (int j = 0; j < kRounds; ++j) {
+      const int h = hb + j * SLOTS + h0;
+      if (hb + j * SLOTS >= heads) break;
+      float4 a = va[j], b = vb[j];
+      const bool is_q = h < p.n_heads, is_k = !is_q && h < p.n_heads + p.n_kv;
+      const float* gamma = is_q ? p.q_gamma : (is_k ? p.k_gamma : nullptr);
+      float ss = a.x * a.x + a.y * a.y + a.z * a.z + a.w * a.w + b.x * b.x + b.y * b.y + b.z * b.z +
+                 b.w * b.w;
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (h >= heads) continue;
+      if (gamma || (!is_q && !is_k && p.v_norm)) {
+        const float r = rsqrtf(ss * (1.0f / HD) + p.eps);
+        float4 ga = make_float4(1.f, 1.f, 1.f, 1.f), gb = ga;
+        if (gamma) {
+          ga = *reinterpret_cast<const float4*>(gamma + 4 * li);
+          gb = *reinterpret_cast<const float4*>(gamma + HD / 2 + 4 * li);
+        }
+        a = make_float4(a.x * r * ga.x, a.y * r * ga.y, a.z * r * ga.z, a.w * r * ga.w);
+        b = make_float4(b.x * r * gb.x, b.y * r * gb.y, b.z * r * gb.z, b.w * r * gb.w);
+      }
+      if (is_q || is_k) {
+        const float4 u = a;
+        a = make_float4(u.x * ca.x - b.x * ca.y, u.y * ca.z - b.y * ca.w, u.z * cb.x - b.z * cb.y,
+                        u.w * cb.z - b.w * cb.w);
+        b = make_float4(b.x * ca.x + u.x * ca.y, b.y * ca.z + u.y * ca.w, b.z * cb.x + u.z * cb.y,
+                        b.w * cb.z + u.w * cb.w);
+      }
+      if (is_q) {
+        const long long o = (long long)row * p.ldq + (long long)h * HD + 4 * li;
+        store4<QF16>(p.q_out, o, a);
+        store4<QF16>(p.q_out, o + HD / 2, b);
+      } else if (put) {
+        const int kvh = is_k ? h - p.n_heads : h - p.n_heads - p.n_kv;
+        uint16_t* pages = is_k ? p.k_pages : p.v_pages;
+        const long long o = ((slot / 16 * p.n_kv + kvh) * 16 + slot % 16) * HD + 4 * li;
+        *reinterpret_cast<uint2*>(pages + o) = pack4(a);
+        *reinterpret_cast<uint2*>(pages + o + HD / 2) = pack4(b);
+      }
     }
   }
 }
