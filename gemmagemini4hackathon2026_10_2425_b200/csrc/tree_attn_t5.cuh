@@ -120,6 +120,9 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* tm, in
       "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
       : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* tm) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tm)) : "memory");
+}
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
 // 128-byte swizzled operands.  K-major (Q, K): 8-row groups 1024 bytes apart.  MN-major (V, whose
@@ -228,8 +231,10 @@ __device__ void steps_prefix(const Params& p, int G, int stride, int* prefix, Sc
     for (int w = 0; w < warp; ++w) base += sc.wsum[w];
     if (j < groups) prefix[j + 1] = base + x;
     __syncthreads();
-    if (tid == threads - 1) sc.carry = base + x;
-    __syncthreads();
+    if (j0 + threads < groups) {
+      if (tid == threads - 1) sc.carry = base + x;
+      __syncthreads();
+    }
   }
 }
 
@@ -412,6 +417,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&mi.q_empty, 1);
     mi.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (tid == 32) {
+    prefetch_map(&p.tmK);
+    prefetch_map(&p.tmV);
+    if (q_tma) prefetch_map(&p.tmQ);
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&mi.tmem)),
@@ -897,20 +907,29 @@ __global__ void __launch_bounds__(256) tree_join_t5_kernel(const Params p, int c
   float top = -INFINITY, total = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int c = blockIdx.x; c <= sp.last; ++c) {
-    if (none(c)) continue;
-    const long long st = state(c);
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + st * 2);
-    float v[E];
+  for (int c0 = blockIdx.x; c0 <= sp.last; c0 += 4) {  // four pieces' loads at a time
+    float2 ml[4];
+    float v[4][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = p.part_o[st * HD + e * 32 + lane];
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;  // nothing seen in this piece
-    const float m = fmaxf(top, ml.x), base = m == -INFINITY ? 0.f : m;
-    const float w0 = ex2(top - base), w1 = ex2(ml.x - base);
-    top = m;
-    total = total * w0 + ml.y * w1;
+    for (int k = 0; k < 4; ++k) {
+      const int c = c0 + k;
+      ml[k] = make_float2(-INFINITY, 0.f);
+      if (c > sp.last || none(c)) continue;
+      const long long st = state(c);
+      ml[k] = *reinterpret_cast<const float2*>(p.part_ml + st * 2);
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * w0 + v[e] * w1;
+      for (int e = 0; e < E; ++e) v[k][e] = p.part_o[st * HD + e * 32 + lane];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;  // nothing seen in this piece, or no piece
+      const float m = fmaxf(top, ml[k].x), base = m == -INFINITY ? 0.f : m;
+      const float w0 = ex2(top - base), w1 = ex2(ml[k].x - base);
+      top = m;
+      total = total * w0 + ml[k].y * w1;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = acc[e] * w0 + v[k][e] * w1;
+    }
   }
   const float inv = total == 0.f ? 0.f : 1.0f / total;
   const long long at = (long long)(sp.row0 + t) * p.ldout + (long long)(sp.kvh * G + (sp.m0 + rr) % G) * HD;
@@ -927,7 +946,7 @@ static bool serves(int head_dim, long long max_steps) {
 // tile then serves two row tiles), unless hi + lo planes need the room.
 struct Shape {
   bool mt2;
-  int rows, m_tiles, grid, stride;
+  int rows, live_rows, m_tiles, grid, stride;  // live_rows: of a unit, at most
   long long max_steps;
   size_t off_ml, off_splits, bytes;
 };
@@ -936,6 +955,7 @@ static Shape shape_of(int batch, int n_heads, int n_kv, int head_dim, int max_q,
   const long long m = (long long)max_q * (n_heads / n_kv);
   h.mt2 = !x2 && m > 128;
   h.rows = h.mt2 ? 256 : 128;
+  h.live_rows = (int)std::min<long long>(m, h.rows);
   h.m_tiles = (int)((m + h.rows - 1) / h.rows);
   const int keys = h.mt2 ? kKeys : 2 * kKeys;
   // + 1: with a window, a unit's first tile may begin anywhere
@@ -958,7 +978,7 @@ static int launch(Params& p, const Shape& h, cudaStream_t stream) {
   B2D_TRY(allow_smem(kern, smem, done));
   kern<<<h.grid, kThreads, smem, stream>>>(p, h.stride);
   B2D_TRY(launch_status());
-  return launch_pdl(tree_join_t5_kernel<HD, C::ROWS>, dim3(h.grid, C::ROWS / 8), dim3(256), 0, stream, p, h.grid);
+  return launch_pdl(tree_join_t5_kernel<HD, C::ROWS>, dim3(h.grid, (h.live_rows + 7) / 8), dim3(256), 0, stream, p, h.grid);
 }
 
 }  // namespace t5
