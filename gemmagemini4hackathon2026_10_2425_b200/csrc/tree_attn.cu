@@ -9,16 +9,22 @@
 //   O_t = sum_j p_tj v_j / sum_j p_tj,   p_tj = exp(scale q_t . k_j - m_t)   over the places seen.
 //
 // The T_b * G query rows of one KV head (G = heads per KV head) are the M side of two tensor-core
-// products per key tile, so each K/V byte of the cache is read once per 64 rows.
+// products per key tile.  head_dim 64 and 128 run on tcgen05 (tree_attn_t5.cuh: 128 or 256 rows
+// share each read of the cache); head_dim 256, whose output rows and tiles do not fit that
+// kernel's TMEM and shared memory, runs on the kernel of this file:
 //  * one CTA per (chunk of keys, 64-row tile of a KV head, sequence): four consumer warps of 16
 //    rows each and one producer warp that streams key tiles (64 keys = 4 pages, TMA, 128-byte
 //    swizzle) through a shared-memory ring;
 //  * S = Q K^T and O += P V on mma.sync m16n8k16, running maximum and sum in registers;
-//  * fp32 q (or an fp32 output) carries q and p as hi + lo fp16 pairs (22 bits), as the decode
-//    attention does: two MMAs for one;
 //  * a sequence cut into several chunks leaves (max, sum, unnormalized output) per row and chunk
-//    in the workspace and a second kernel joins them; no state survives a call, so the workspace
-//    needs no initial contents and calls on different streams share nothing.
+//    in the workspace and a second kernel joins them.
+// Measured for 8 trees of 64 nodes over 8k-32k places at head_dim 128: 874 us on mma.sync, 197 us
+// on tcgen05; for one draft of 8 rows over 1021 places 43.7 and 16 us.  So every size goes to
+// tcgen05 where it can.
+//
+// fp32 q (or an output wider than fp16) carries q and the weights as hi + lo fp16 pairs (22 bits),
+// as the decode attention does: two MMAs for one.  No state survives a call, so the workspace
+// needs no initial contents and calls on different streams share nothing.
 //
 // Places a row must not see contribute nothing whatever they hold: scores are replaced, not
 // added to, and a tile that any row sees only in part has its V checked -- rows past the end are
@@ -42,7 +48,7 @@ constexpr int kWarps = 4;                       // consumer warps
 constexpr int kThreads = 32 * kWarps + 32;      // + the producer warp
 constexpr int kRows = 16 * kWarps;              // query rows (t, g) per CTA
 constexpr int kKeys = 64;                       // keys per tile
-constexpr int kMaxChunk = 4096;                 // keys per CTA
+constexpr int kMaxChunk = 32768;                // keys per CTA (their page ids are in shared memory)
 constexpr int kMaxWords = 8;
 
 __device__ int g_error;  // a bounded wait gave up (b2d_paged_tree_attn_error)
@@ -119,7 +125,7 @@ template <int HD>
 struct Cfg {
   static constexpr int BOXES = HD / 64;
   static constexpr int TILE = kKeys * HD * 2;  // one K (or V) tile
-  static constexpr int STAGES = HD == 256 ? 2 : 3;
+  static constexpr int STAGES = 2;
   static constexpr int Q_PLANE = kRows * HD * 2;
   static constexpr int SMEM(bool x2) {
     return 1024 + STAGES * 2 * TILE + (x2 ? 2 : 1) * Q_PLANE + kMaxChunk / 16 * 4;
@@ -652,12 +658,12 @@ static bool shape_ok(int batch, int rows, int n_heads, int n_kv, int max_q, int 
 size_t paged_tree_attn_workspace_bytes(int batch, int rows, int n_heads, int n_kv_heads, int head_dim,
                                        int max_q, int max_ctx) {
   if (!tree::shape_ok(batch, rows, n_heads, n_kv_heads, max_q, max_ctx) || head_dim <= 0) return 0;
+  if (head_dim == 256)
+    return tree::plan_of(batch, rows, n_heads, n_kv_heads, head_dim, max_q, max_ctx).bytes;
   size_t need = 0;
   for (const bool x2 : {false, true}) {
     const tree::t5::Shape h = tree::t5::shape_of(batch, n_heads, n_kv_heads, head_dim, max_q, max_ctx, x2);
-    need = std::max(need, tree::t5::serves(head_dim, h.max_steps)
-                              ? h.bytes
-                              : tree::plan_of(batch, rows, n_heads, n_kv_heads, head_dim, max_q, max_ctx).bytes);
+    if (h.max_steps < (1ll << 31)) need = std::max(need, h.bytes);
   }
   return need;
 }
@@ -684,6 +690,9 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) ||
       ldq % (q_dtype == B2D_F16 ? 8 : 4) || ldout % (out_dtype == B2D_F32 ? 4 : 8))
     return B2D_ERR_ALIGN;
+  const bool x2 = q_dtype == B2D_F32 || out_dtype != B2D_F16;
+  const tree::t5::Shape h = tree::t5::shape_of(batch, n_heads, n_kv_heads, head_dim, max_q, max_ctx, x2);
+  if (head_dim != 256 && h.max_steps >= (1ll << 31)) return B2D_ERR_SHAPE;  // steps are counted in 32 bits
   const size_t need =
       paged_tree_attn_workspace_bytes(batch, rows, n_heads, n_kv_heads, head_dim, max_q, max_ctx);
   if (need && (!workspace || workspace_bytes < need)) return B2D_ERR_WORKSPACE;
@@ -716,9 +725,7 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
   p.out_lo = out_dtype == B2D_F16X2 ? static_cast<uint16_t*>(out) + (size_t)rows * ldout : nullptr;
   p.ldout = ldout;
   p.part_o = static_cast<float*>(workspace);
-  const bool x2 = q_dtype == B2D_F32 || out_dtype != B2D_F16;
-  const tree::t5::Shape h = tree::t5::shape_of(batch, n_heads, n_kv_heads, head_dim, max_q, max_ctx, x2);
-  if (tree::t5::serves(head_dim, h.max_steps)) {
+  if (head_dim != 256) {
     B2D_TRY(make_tmap_f16_blocks(&p.tmV, v_pages, prows, head_dim, 16));
     const int G = n_heads / n_kv_heads;
     if (p.q_f16 && 128 % G == 0)
@@ -740,14 +747,8 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
   p.chunk = pl.chunk;
   p.max_chunks = pl.max_chunks;
   p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.off_ml);
-  switch (head_dim) {
-    case 64: return x2 ? tree::launch<64, true>(p, pl.m_tiles, batch, stream)
-                       : tree::launch<64, false>(p, pl.m_tiles, batch, stream);
-    case 128: return x2 ? tree::launch<128, true>(p, pl.m_tiles, batch, stream)
-                        : tree::launch<128, false>(p, pl.m_tiles, batch, stream);
-    default: return x2 ? tree::launch<256, true>(p, pl.m_tiles, batch, stream)
-                       : tree::launch<256, false>(p, pl.m_tiles, batch, stream);
-  }
+  return x2 ? tree::launch<256, true>(p, pl.m_tiles, batch, stream)
+            : tree::launch<256, false>(p, pl.m_tiles, batch, stream);
 }
 
 int paged_tree_attn_error() {

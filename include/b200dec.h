@@ -394,17 +394,20 @@ B2D_API int b2d_qk_norm_rope_append(const void* qkv, int qkv_dtype, int ldqkv,
  * with its bit set in mask[row][mask_words] (a drafted tree; mask_words <= 8), or with mask NULL
  * the rows up to itself.  window > 0 further hides every place whose position is <= the row's
  * position - window: positions are the places themselves, except that with a mask the step's own
- * rows have positions[row] (required then; b2d_paged_plan's).  A row that sees nothing gives
- * zeros.  What a hidden place holds (infinities and NaN included) changes nothing.
- * out [rows, Hq * HD] (F32, F16 or F16X2 with its lo plane at out + rows * ldout).  fp16 q with an
- * fp16 output multiplies in fp16 with fp32 sums; every other combination carries q and the
- * weights as hi + lo fp16 pairs.  head_dim 64, 128 or 256; n_heads / n_kv_heads <= 64.
+ * rows have positions[row] (required then; b2d_paged_plan's: row i's is held to ctx_lens[b] ..
+ * ctx_lens[b] + i).  A row that sees nothing gives zeros.  What a hidden place holds (infinities
+ * and NaN included) changes nothing.
+ * out [rows, Hq * HD] (F32, F16 or F16X2 with its lo plane at out + rows * ldout; not q itself).
+ * fp16 q with an fp16 output multiplies in fp16 with fp32 sums; every other combination carries q
+ * and the weights as hi + lo fp16 pairs.  head_dim 64, 128 (tcgen05) or 256 (mma.sync);
+ * n_heads / n_kv_heads <= 64.
  * max_q bounds the rows of a sequence and max_ctx every ctx_lens[b] + rows (a sequence beyond
  * max_ctx, and rows beyond max_q, are left as they were).  Block-table entries outside
  * [0, n_blocks) are never dereferenced; their places are hidden.  scale <= 0 means
  * 1/sqrt(head_dim).
  * Workspace: b2d_paged_tree_attn_workspace_bytes() bytes (may be 0), any contents; it holds
- * nothing between calls, and calls that may overlap need one each.
+ * nothing between calls, and calls that may overlap need one each.  Two launches: the attention
+ * and, started dependently, the join of what several CTAs shared.
  * b2d_paged_tree_attn_error waits for the device and returns B2D_ERR_TIMEOUT if a bounded wait of
  * a call on the current device gave up since the last query (its output is incomplete). */
 B2D_API size_t b2d_paged_tree_attn_workspace_bytes(int batch, int rows, int n_heads,

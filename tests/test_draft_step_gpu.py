@@ -367,6 +367,52 @@ def test_attn_many_sequences(hq, hk, hd, q):
     check_attn(c, torch.float32)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attn_large_batch(hd):
+    """More sequences than prefix sums are kept for, many of them without rows."""
+    r = np.random.default_rng(hd)
+    c = attn_case(hd, r.integers(0, 40, 900), r.integers(0, 3, 900), 2, 1, hd, False)
+    check_attn(c, torch.float16)
+
+
+def test_attn_two_calls_at_once():
+    """Two streams, each with its own call in flight: nothing is shared between them."""
+    cases = [attn_case(20 + i, [4000, 900], [30, 9], 8, 2, 128, True) for i in range(2)]
+    want = [run_attn(c, torch.float16) for c in cases]
+    args = [(gpu(c["q"]), gpu(c["kp"]), gpu(c["vp"]), gpu(c["table"]), gpu(c["ctx"]), gpu(c["cu"]), *c["dims"], c["max_q"], c["max_ctx"])
+            for c in cases]
+    masks = [gpu(c["mask"]) for c in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(ops.paged_tree_attn(*args[i], mask=masks[i], out_dtype=torch.float16))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+def test_attn_fp16_rows_to_planes():
+    c = attn_case(16, [300, 2], [9, 70], 16, 4, 64, True)
+    want = run_attn(c)
+    x2 = torch.zeros(2, c["R"], 16 * 64, dtype=torch.float16, device=DEV)
+    run_attn(c, out=x2)
+    err = (ops.from_f16x2(x2) - want).abs()
+    assert torch.all(err <= 2.0**-21 * want.abs() + 2.0**-24)
+
+
+def test_attn_positions_are_held_to_the_tree():
+    """Given positions below the context or past a row's own place count as those."""
+    c = attn_case(17, [60, 7], [12, 5], 4, 2, 64, True)
+    c["pos"] = np.where(np.arange(c["R"]) % 2 == 0, -5, 10**6).astype(np.int32)
+    got = run_attn(c, window=30)
+    own = np.concatenate([np.arange(12), np.arange(5)])
+    c["pos"] = np.where(np.arange(c["R"]) % 2 == 0, np.repeat(c["ctx"], [12, 5]), np.repeat(c["ctx"], [12, 5]) + own).astype(np.int32)
+    assert torch.equal(got, run_attn(c, window=30))
+    check_attn(c, torch.float32, window=30)
+
+
 def test_attn_widest_tree():
     check_attn(attn_case(8, [37], [256], 4, 2, 64, True), torch.float16)
 
