@@ -247,6 +247,18 @@ class DecodeEngine:
 
     # -- step -------------------------------------------------------------------------------
 
+    def _take(self, *tensors: torch.Tensor | None) -> None:
+        """Order self.stream after the caller's current stream, which made the tensors, and keep their
+        memory from being handed out again while a step still reads it (a caller that makes new ones
+        for every step runs ahead of the GPU).  Nothing to do for a caller on self.stream."""
+        cur = torch.cuda.current_stream(self.device)
+        if cur == self.stream:
+            return
+        self.stream.wait_stream(cur)
+        for t in tensors:
+            if t is not None:
+                t.record_stream(self.stream)
+
     def step(
         self,
         tokens: torch.Tensor,
@@ -264,6 +276,7 @@ class DecodeEngine:
                 raise ValueError("tokens, ctx_lens, block_table, next_tokens: contiguous CUDA int32")
         if block_table.shape != (B, self.max_blocks):
             raise ValueError(f"block_table must be [{B}, {self.max_blocks}]")
+        self._take(tokens, ctx_lens, block_table, next_tokens, logits)
         call(
             "b2d_decoder_step",
             self._h,
@@ -298,6 +311,7 @@ class DecodeEngine:
             ring = torch.zeros(max(n_steps, 1), B, dtype=torch.int32, device=tokens.device)
         if ring_count is None:
             ring_count = torch.zeros(1, dtype=torch.int32, device=tokens.device)
+        self._take(tokens, ctx_lens, block_table, ring, ring_count)
         call(
             "b2d_decoder_generate",
             self._h,
@@ -336,6 +350,7 @@ class DecodeEngine:
             next_token = torch.empty(1, dtype=torch.int32, device=tokens.device)
         if logits is not None and (logits.dtype != torch.float32 or logits.numel() < self.lm_rows):
             raise ValueError(f"logits must be fp32 with >= {self.lm_rows} elements")
+        self._take(tokens, seq_table, next_token, logits)
         call(
             "b2d_decoder_prefill",
             self._h,
