@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     return more;
   };
   bool dead = false;
-  int kc = 0, vc = 0;  // tiles through the rings so far (every role counts them alike)
+  int kc = 0, vc = 0;  // tiles (warp 11: units) through the rings so far; every role counts them alike
   auto wait = [&](uint64_t* bar, uint32_t phase) {
     // after a wait that gave up nobody waits any more, but every role runs to its end
     if (!dead && !mbar_wait(bar, phase, &g_error, 1)) {
@@ -496,9 +496,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-      }
-      if (*reinterpret_cast<volatile int*>(&mi.failed)) {  // copies in flight land before the CTA ends
-        for (int i = max(0, kc - stages); i < kc; ++i) mbar_wait(&full[i % stages], (i / stages) & 1, &g_error, 1);
       }
     } else if (warp == 9) {
       // ---------------- MMA: one elected lane, the warpgroups in turn ----------------
@@ -606,10 +603,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (q_tma) {
       // ---------------- TMA: Q, as soon as the scores of the unit before are formed ----------------
-      int nq = 0;
       while (next_warp()) {
-        if (nq > 0) wait(&mi.q_empty, (nq - 1) & 1);
-        ++nq;
+        if (kc > 0) wait(&mi.q_empty, (kc - 1) & 1);
+        ++kc;
         if (lane == 0) {
           constexpr int TILES = MT2 ? 2 : 1;
           mbar_expect_tx(&mi.q_full, TILES * C::TILE);
@@ -619,7 +615,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                           pc.s.row0 + (pc.m0 + g * 128) / G, bx, &mi.q_full);
         }
       }
-      if (*reinterpret_cast<volatile int*>(&mi.failed) && nq > 0) mbar_wait(&mi.q_full, (nq - 1) & 1, &g_error, 1);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
@@ -887,6 +882,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before();
   __syncthreads();
   fence_after();
+  if (mi.failed) {  // a wait gave up somewhere: copies in flight land before the CTA ends
+    const bool k = warp == 8;
+    const int stages = k ? C::SK : C::SV;
+    if (k || warp == 10)
+      for (int i = max(0, kc - stages); i < kc; ++i)
+        mbar_wait(&(k ? mi.k_full : mi.v_full)[i % stages], (i / stages) & 1, &g_error, 1);
+    if (warp == 11 && q_tma && kc > 0) mbar_wait(&mi.q_full, (kc - 1) & 1, &g_error, 1);
+    __syncthreads();
+  }
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
 }

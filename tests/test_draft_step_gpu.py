@@ -77,7 +77,7 @@ def check_plan(c, R=None):
     return w
 
 
-@pytest.mark.parametrize("B,ctx_hi,q_hi", [(1, 0, 1), (1, 40, 1), (5, 100, 3), (33, 500, 40), (513, 300, 2), (700, 60, 65), (2000, 17, 1)])
+@pytest.mark.parametrize("B,ctx_hi,q_hi", [(1, 0, 1), (1, 40, 1), (5, 100, 3), (33, 500, 40), (513, 300, 2), (700, 60, 65), (2000, 17, 1), (8192, 40, 2)])
 @pytest.mark.parametrize("short", [False, True])
 def test_plan(B, ctx_hi, q_hi, short):
     check_plan(plan_case(B + q_hi, B, ctx_hi, q_hi, short=short))
