@@ -7,7 +7,9 @@
 // both online: when a thread's maximum grows from m to m', s <- s e^(m-m'), and u likewise with
 // (m - m') s added to it.  Work is done in units of log2 (z = x * L - M with L = fp32(log2 e) and
 // M an fp32 number near max * L); the result is exact in M, and the relative error of L (1e-8)
-// is a relative error of the results.
+// is a relative error of the results.  z of the maximum itself is what rounding max * L left over,
+// up to half a step of M, so this form serves |max| < 2^24 only, where that is below 1; other rows
+// are summed again as x - max (2^z of a rounding error beyond 128 is infinite: |max| >= 1.5e9).
 //
 // Top k without a second pass over the row: every thread remembers its own largest value and the
 // vector it came from (one compare per vector of the main loop).  The k-th largest of the maxima
@@ -36,10 +38,13 @@ constexpr int kGroup = kThreads / 64;  // threads per group of the bound
 constexpr int kCand = 1024;  // candidates ranked at once; more of them take the slow way
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr double kLn2 = 0.693147180559945309417;
-// Values below -2^100 count as -2^100 in the sums, which keeps 0 * inf out of u (their weight is
-// zero either way, unless the whole row is that low; such rows are summed again).  A power of
-// two, so that kFloor * kLog2e is exact and a vector of nothing else has z = 0.
-constexpr float kFloor = -1.2676506002282294e30f;
+// Values below -2^24 count as -2^24 in the sums: a thread that has seen nothing above it (tokens
+// banned with any constant) then has a reference without a rounding error, and 0 * inf stays out of
+// u.  Their weight is zero either way in a row whose maximum is kReach or more above the floor;
+// lower rows are summed again.  A power of two, so that kFloor * kLog2e is exact and a vector of
+// nothing else has z = 0.
+constexpr float kFloor = -16777216.f;
+constexpr float kReach = 256.f;  // e^-256 is nothing in fp32
 
 struct Params {
   const void* x;
@@ -275,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Param
     __syncthreads();
     const unsigned long long tau = g_tau;
     const float tau_v = key_value(tau);
-    bool odd = false;  // a NaN (or an infinite maximum): the thread maxima say nothing
+    bool odd = false;  // a NaN (or a maximum past 1.5e9): the thread maxima may say nothing
     for (int w = 0; w < kWarps; ++w) odd |= w_stat[w].s != w_stat[w].s;
     // threads that may hold an element at or above tau
     if (mv >= 0 && key_of(mx, (unsigned)max(r.first(mv), 0)) >= tau)
@@ -347,12 +352,11 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Param
   if (rank != 0) return;
   Stat t = r_stat[0];
   for (int j = 1; j < ranks; ++j) t = join(t, r_stat[j]);
-  // Rows whose maximum is outside [-2^100, 2e38], all of them -inf included: the plain two-step
-  // form x - max, over the whole row by this CTA.
+  // Rows whose maximum is not within (-2^24 + 256, 2^24), all of them -inf included: the plain
+  // two-step form x - max, over the whole row by this CTA.  (Their sums may be infinite or NaN here.)
   float base = 0.f;
-  const bool odd = t.s == t.s && !(t.M > kFloor * kLog2e);
-  const bool huge = !(t.M < 2.9e38f);
-  if (odd || huge) {
+  const bool far = !(t.M > (kFloor + kReach) * kLog2e && t.M < -kFloor * kLog2e);
+  if (far) {
     float m = -INFINITY;
     for (int v = tid; v < r.nv; v += kThreads) {
       float f[VEC];
@@ -381,7 +385,6 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Param
     for (int w = 1; w < kWarps; ++w) t = join(t, w_stat[w]);
     if (base == -INFINITY) t = Stat{0.f, 1.f, 0.f};  // nothing but -inf: no choice, entropy 0
   }
-  const bool far = odd || huge;
   // log2 of the row's sum, in log2 units of x * L (of (x - base) * L in a far row)
   __shared__ double row_lz;
   if (tid == 0) {
