@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
   uint8_t* qs = ring + C::STAGES * 2 * C::TILE;  // [planes][BOXES][64 rows][128 bytes]
   int* blk = reinterpret_cast<int*>(qs + (X2 ? 2 : 1) * C::Q_PLANE);
   __shared__ __align__(8) uint64_t full[C::STAGES], empty[C::STAGES];
-  __shared__ unsigned long long bad_keys;
+  __shared__ unsigned long long bad_keys[3];  // non-finite V rows of a looked-over tile, in turn
   __shared__ int failed;
 
   const int G = p.n_heads / p.n_kv;
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed = 0;
-    bad_keys = 0;
+    bad_keys[0] = bad_keys[1] = bad_keys[2] = 0ull;
   }
   // q rows of the tile into shared memory, as fp16 (hi and lo parts of fp32)
   for (int i = tid; i < kRows * (HD / 8); i += kThreads) {
@@ -345,6 +345,7 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
     float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
     const uint32_t qb = smem_u32(qs);
     bool dead = false;
+    int nl = 0;  // tiles looked over
 
     for (int i = 0; i < tiles; ++i) {
       const int st = i % C::STAGES, j0 = lo + i * kKeys;
@@ -361,26 +362,30 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
       for (int pg = 0; pg < kKeys / 16; ++pg) whole &= blk[i * (kKeys / 16) + pg] >= 0;
       unsigned long long bad = 0ull;
       if (!whole) {
-        // zero the V rows past the end or without a page; find and zero non-finite ones
+        // zero the V rows past the end or without a page; find and zero non-finite ones.  A warp may
+        // be a tile ahead of another between two barriers, so three words take turns: the next
+        // tile's is cleared before this tile's barrier, when everyone is past the tile that used it
+        unsigned long long* const found = &bad_keys[nl % 3];
         for (int x = tid; x < kKeys * (HD / 8); x += 32 * kWarps) {
           const int r = x / (HD / 8), ch = x % (HD / 8);
           uint4* v = reinterpret_cast<uint4*>(Vt + sw(r, ch, kKeys));
           const bool out = j0 + r >= s.hi || blk[i * (kKeys / 16) + r / 16] < 0;
           if (!out) {
-            if (nonfinite(*v)) atomicOr(&bad_keys, 1ull << r);
+            if (nonfinite(*v)) atomicOr(found, 1ull << r);
           } else {
             *v = make_uint4(0u, 0u, 0u, 0u);
           }
         }
+        if (tid == 0) bad_keys[(nl + 1) % 3] = 0ull;
+        ++nl;
         consumers_sync();
-        bad = *reinterpret_cast<volatile unsigned long long*>(&bad_keys);
+        bad = *reinterpret_cast<volatile unsigned long long*>(found);
         if (bad) {  // whole rows of V go, finite elements too: bad rows are added by hand
           for (int x = tid; x < kKeys * (HD / 8); x += 32 * kWarps) {
             const int r = x / (HD / 8), ch = x % (HD / 8);
             if ((bad >> r) & 1) *reinterpret_cast<uint4*>(Vt + sw(r, ch, kKeys)) = make_uint4(0u, 0u, 0u, 0u);
           }
           consumers_sync();
-          if (tid == 0) bad_keys = 0ull;
         }
       }
 

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_draft_step_gpu import DEV, check_score
+from test_draft_step_gpu import DEV, attn_case, check_attn, check_score
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,38 @@ def test_score_around_the_floor():
         x[i, 17] = -(2.0**24) + m
         x[i, 99] = -(2.0**24) + m - 2
     check_score(x, score_targets(6, 5000), 5)
+
+
+# -- paged_tree_attn ----------------------------------------------------------------------------
+
+
+def spoil(c, b, places, part, fill, heads=slice(None)):
+    for j in places:
+        c[part][c["table"][b, j // 16], heads, j % 16, 5] = fill
+
+
+@pytest.mark.parametrize("hd", [256])
+@pytest.mark.parametrize("fill", [np.nan, np.inf])
+def test_attn_hidden_rows_of_many_tiles(hd, fill):
+    """Every tile of a wide tree holds places that some rows must not see, and in most of them v (every
+    other tile: none, one or several rows) is not finite."""
+    for T, ctx in ((256, 40), (200, 0)):
+        c = attn_case(hd + T, [ctx, 9], [T, 3], 4, 2, hd, True)
+        for tile in (0, 1, 3):
+            spoil(c, 0, ctx + 64 * tile + np.arange(5, 5 + 3 * (tile + 1), 3), "vp", fill, tile % 2)
+        spoil(c, 0, [ctx + 130], "kp", fill)
+        check_attn(c, torch.float16)
+        check_attn(c, torch.float32)
+
+
+@pytest.mark.parametrize("hd", [256])
+def test_attn_window_of_many_tiles(hd):
+    """Chunks whose window cuts through every tile that they read; what left it, and every page's unused
+    part, is not finite."""
+    for window in (30, 200):
+        c = attn_case(hd + window, [700, 90], [150, 70], 4, 2, hd, False)
+        spoil(c, 0, range(700 - window), "vp", np.inf)
+        spoil(c, 0, range(700 - window), "kp", np.nan)
+        spoil(c, 0, [701, 790, 840], "vp", np.nan, 1)
+        check_attn(c, torch.float16, window=window)
+        check_attn(c, torch.float32, window=window)
