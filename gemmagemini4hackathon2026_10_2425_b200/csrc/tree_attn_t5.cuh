@@ -442,11 +442,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   Piece& pc = mi.pc[warp];
   if (lane == 0) mi.walk[warp].begin(p, mi.prefix, stride, W);
   auto next_warp = [&]() {
-    __syncwarp();
+    __syncwarp();  // the lanes are done with the piece before
     bool more = false;
     if (lane == 0) more = mi.walk[warp].next(p, G, pc);
-    more = __shfl_sync(0xffffffffu, (int)more, 0) != 0;
-    return more;
+    __syncwarp();  // and see the next one: a shuffle orders no memory
+    return __shfl_sync(0xffffffffu, (int)more, 0) != 0;
   };
   bool dead = false;
   int kc = 0, vc = 0;  // tiles (warp 11: units) through the rings so far; every role counts them alike

@@ -66,7 +66,7 @@ def spoil(c, b, places, part, fill, heads=slice(None)):
         c[part][c["table"][b, j // 16], heads, j % 16, 5] = fill
 
 
-@pytest.mark.parametrize("hd", [256])
+@pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("fill", [np.nan, np.inf])
 def test_attn_hidden_rows_of_many_tiles(hd, fill):
     """Every tile of a wide tree holds places that some rows must not see, and in most of them v (every
@@ -80,7 +80,7 @@ def test_attn_hidden_rows_of_many_tiles(hd, fill):
         check_attn(c, torch.float32)
 
 
-@pytest.mark.parametrize("hd", [256])
+@pytest.mark.parametrize("hd", [64, 128, 256])
 def test_attn_window_of_many_tiles(hd):
     """Chunks whose window cuts through every tile that they read; what left it, and every page's unused
     part, is not finite."""
