@@ -336,6 +336,7 @@ __device__ __forceinline__ void add_place(const Params& p, int b, int kvh, int j
 #pragma unroll
     for (int e = 0; e < 32; ++e)
       if (w != 0.f) o[e] = __float_as_uint(fmaf(w, h2f(v[c + e]), __uint_as_float(o[e])));
+    __syncwarp();
     tmem_st32(o_col + c, o);
   }
   tmem_wait_st();
@@ -681,6 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               if ((miss >> (2 * w)) & 1) see[w] &= 0xffff0000u;
               if ((miss >> (2 * w + 1)) & 1) see[w] &= 0x0000ffffu;
             }
+            __syncwarp();  // the lanes' branches end here: TMEM is read by the whole warp at once
           }
           float x[kKeys];
 #pragma unroll
@@ -856,16 +858,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             tmem_wait_ld();
           }
-          if (!live) continue;
-          if (pc.whole) {
+          if (live && pc.whole) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] *= inv;
             store_row32(p, (long long)(s.row0 + t) * p.ldout + (long long)head * HD + c0 + cc, o);
-          } else {
+          } else if (live) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
               *reinterpret_cast<float4*>(part + cc + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
+          __syncwarp();  // rows that are not live come along: TMEM is read by the whole warp at once
         }
         if (!pc.whole && live && (MT2 || g == 0))
           *reinterpret_cast<float2*>(p.part_ml + ((long long)pc.slot * C::ROWS + (m - pc.m0)) * 2) =
