@@ -303,6 +303,7 @@ struct Misc {
   float2 ml[2][MT2 ? 1 : 128];  // key split: the warpgroups' (reference, sum) per row
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
   uint64_t s_full[2], p_full[2], pv_done[2], q_full, q_empty, v_seen[2];
+  uint64_t drained;             // after a wait that gave up: every MMA issued has ended
   unsigned bad[2][3][4];        // non-finite V rows of a tile that was looked over
   uint32_t tmem;
   int failed;
@@ -417,6 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(&mi.q_full, q_tma ? 1 : 8);
     mbar_init(&mi.q_empty, 1);
+    mbar_init(&mi.drained, 1);
     mi.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -504,6 +506,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // tensor cores do that, the other warpgroup has the exponential units to itself, and the two
       // keep alternating.  (Two issuing threads let both warpgroups do the same thing at the same
       // time.)
+      // After a wait that gave up it hands nothing back to the loaders: a barrier with a copy in
+      // flight must not be armed again.
       const uint32_t sm0 = smem_u32(sm);
       int np[2] = {0, 0}, nq = 0;  // products issued per warpgroup, pieces begun
       while (next_warp()) {
@@ -523,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mma_ss(tmem + g * 128, q + pl * (C::TILE >> 4) + o, k + o, idesc(kKeys, false), pl > 0 || e > 0);
               }
             commit(&mi.s_full[g]);
-            if (last) commit(&mi.k_empty[ks]);
+            if (last && !dead) commit(&mi.k_empty[ks]);
           }
           __syncwarp();
         };
@@ -542,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int e = 0; e < kKeys / 16; ++e)
                 mma_ts(tmem + 256 + g * HD, tmem + g * 128 + pl * 64 + e * 8, v + e * (HD * 2), idesc(HD, true));
             commit(&mi.pv_done[g]);
-            if (last) commit(&mi.v_empty[vs]);
+            if (last && !dead) commit(&mi.v_empty[vs]);
           }
           __syncwarp();
         };
@@ -558,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (np[g] > 0) wait(&mi.pv_done[g], (np[g] - 1) & 1);
         fence_after();
         auto q_done = [&]() {  // every score of the unit is on its way: Q may go once they are formed
-          if (elect_one()) commit(&mi.q_empty);
+          if (elect_one() && !dead) commit(&mi.q_empty);
           __syncwarp();
         };
         if constexpr (MT2) {
@@ -606,6 +610,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---------------- TMA: Q, as soon as the scores of the unit before are formed ----------------
       while (next_warp()) {
         if (kc > 0) wait(&mi.q_empty, (kc - 1) & 1);
+        dead = __any_sync(0xffffffffu, dead);
+        if (dead) break;
         ++kc;
         if (lane == 0) {
           constexpr int TILES = MT2 ? 2 : 1;
@@ -884,13 +890,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before();
   __syncthreads();
   fence_after();
-  if (mi.failed) {  // a wait gave up somewhere: copies in flight land before the CTA ends
+  // a wait gave up somewhere: copies and MMAs in flight end before the CTA does
+  if (mi.failed) {
     const bool k = warp == 8;
     const int stages = k ? C::SK : C::SV;
     if (k || warp == 10)
       for (int i = max(0, kc - stages); i < kc; ++i)
         mbar_wait(&(k ? mi.k_full : mi.v_full)[i % stages], (i / stages) & 1, &g_error, 1);
     if (warp == 11 && q_tma && kc > 0) mbar_wait(&mi.q_full, (kc - 1) & 1, &g_error, 1);
+    if (warp == 9) {
+      if (elect_one()) commit(&mi.drained);
+      __syncwarp();
+      mbar_wait(&mi.drained, 0, &g_error, 1);
+    }
     __syncthreads();
   }
   if (warp == 0)
