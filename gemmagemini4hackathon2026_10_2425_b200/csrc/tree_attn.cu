@@ -448,7 +448,8 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
             if (!see) sc[n][e] = -INFINITY;
           }
       }
-      // running maximum and sum, in log2 units
+      // running maximum and sum.  Weights are 2^((s - m) c): a product m c of its own would be off by up
+      // to half a step, which is 2^9 for |m c| near 2^33
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float m = -INFINITY;
@@ -456,15 +457,15 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
         for (int n = 0; n < NT; ++n) m = fmaxf(m, fmaxf(sc[n][2 * h], sc[n][2 * h + 1]));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        m = fmaxf(mx[h], m * p.scale_log2);
+        m = fmaxf(mx[h], m);
         const float base = m == -INFINITY ? 0.f : m;  // nothing seen yet: every weight is 2^-inf
-        const float corr = ex2(mx[h] - base);
+        const float corr = ex2((mx[h] - base) * p.scale_log2);
         mx[h] = m;
         float part = 0.f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          sc[n][2 * h] = ex2(fmaf(sc[n][2 * h], p.scale_log2, -base));
-          sc[n][2 * h + 1] = ex2(fmaf(sc[n][2 * h + 1], p.scale_log2, -base));
+          sc[n][2 * h] = ex2((sc[n][2 * h] - base) * p.scale_log2);
+          sc[n][2 * h + 1] = ex2((sc[n][2 * h + 1] - base) * p.scale_log2);
           part += sc[n][2 * h] + sc[n][2 * h + 1];
         }
         sum[h] = fmaf(sum[h], corr, part);
@@ -567,7 +568,7 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
       mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1, &g_error, 1);
 }
 
-// Joins the chunks of one row of one head: weights 2^(m_c - m), one warp per (row, head).
+// Joins the chunks of one row of one head: weights 2^((m_c - m) c), one warp per (row, head).
 template <int HD>
 __global__ void __launch_bounds__(256) tree_join_kernel(const Params p) {
   const int G = p.n_heads / p.n_kv;
@@ -589,7 +590,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const Params p) {
   for (int e = 0; e < HD / 32; ++e) acc[e] = 0.f;
   for (int c = 0; c < nact; ++c) {
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (pi + c) * 2);
-    const float w = ex2(ml.x - top);
+    const float w = ex2((ml.x - top) * p.scale_log2);
     if (ml.x == -INFINITY && ml.y == 0.f) continue;  // nothing seen in this chunk
     total = fmaf(w, ml.y, total);
 #pragma unroll

@@ -19,6 +19,10 @@
 // Roles: warps 0-7 softmax (warp w reads TMEM lanes 32 (w % 4) ..), warps 8 and 10 load K and V
 // (TMA), warp 9 issues the MMAs, warp 11 loads the next unit's Q while this one ends.
 //
+// Weights are 2^((s - ref) c), c = scale log2(e), ref a score: a product ref c of its own would be off
+// by up to half a step, which is 2^9 for |ref c| near 2^33.  The difference is one more operation per
+// pair of scores than a fused s c - ref c.
+//
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the last time (its
 // weights are then up to 256 and still exact to 2^-11 in fp16), which after the first tiles of a
 // unit is almost never; the sum and the weights always use the same reference, so nothing is lost.
@@ -95,6 +99,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -723,12 +732,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               m4[k] = e + 4 + k < kKeys ? fmaxf(fmaxf(m4[k], x[e + k]), x[e + 4 + k]) : fmaxf(m4[k], x[e + k]);
-          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
-          const bool grow = mx > ref + kSlack || (ref == -INFINITY && mx > -INFINITY);
+          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          // (the first place seen: inf > kSlack; none yet: NaN > kSlack)
+          const bool grow = (mx - ref) * p.scale_log2 > kSlack;
           if (__any_sync(0xffffffffu, grow)) {
-            const float to = grow ? mx : ref;
-            const float corr = to == -INFINITY ? 1.f : ex2(ref - to);
-            ref = to;
+            const float corr = grow ? ex2((ref - mx) * p.scale_log2) : 1.f;
+            if (grow) ref = mx;
             sum *= corr;
             if (i >= PER) {  // O holds something; this tile's scores being there, its product is done
 #pragma unroll
@@ -754,7 +763,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < 16; ++e) {
               float& x0 = x[32 * h + 2 * e];
               float& x1 = x[32 * h + 2 * e + 1];
-              const float2 z = split(fma2(two(x0, x1), c2, b2));
+              const float2 z = split(mul2(add2(two(x0, x1), b2), c2));
               x0 = ex2(z.x);
               x1 = ex2(z.y);
               acc[e & 1] = add2(acc[e & 1], two(x0, x1));
@@ -841,8 +850,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float2 a = mi.ml[0][r], b = mi.ml[1][r];
         ref = fmaxf(a.x, b.x);
         const float base = ref == -INFINITY ? 0.f : ref;
-        w0 = ex2(a.x - base);
-        w1 = ex2(b.x - base);
+        w0 = ex2((a.x - base) * p.scale_log2);
+        w1 = ex2((b.x - base) * p.scale_log2);
         sum = a.y * w0 + b.y * w1;
       }
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // no place seen: zeros
@@ -943,7 +952,7 @@ __global__ void __launch_bounds__(256) tree_join_t5_kernel(const Params p, int c
     for (int k = 0; k < 4; ++k) {
       if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;  // nothing seen in this piece, or no piece
       const float m = fmaxf(top, ml[k].x), base = m == -INFINITY ? 0.f : m;
-      const float w0 = ex2(top - base), w1 = ex2(ml[k].x - base);
+      const float w0 = ex2((top - base) * p.scale_log2), w1 = ex2((ml[k].x - base) * p.scale_log2);
       top = m;
       total = total * w0 + ml[k].y * w1;
 #pragma unroll

@@ -6,7 +6,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_draft_step_gpu import DEV, attn_case, check_attn, check_score
+from oracle import ops as O
+from test_draft_step_gpu import DEV, E16, E32, TINY16, attn_case, check_attn, check_score, run_attn, tree_clean
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +92,64 @@ def test_attn_window_of_many_tiles(hd):
         spoil(c, 0, [701, 790, 840], "vp", np.nan, 1)
         check_attn(c, torch.float16, window=window)
         check_attn(c, torch.float32, window=window)
+
+
+def check_exact_scores(c, out_dtype, scale, lost=None):
+    """Rows whose scores are exact in fp32 and the largest of a row's far weights 2^-64 or nothing.  A weight
+    is off by the roundings of z = (s - m) c, |z| <= 64: the difference, the product and c, 2^-24 each (times
+    ln 2), and the exponential's 2^-22; then by E16 where it is an fp16 number, 2^-21 as two; `lost` is what
+    places of small weight may lose.  Sums over n places: one step per 16."""
+    hq, hk, hd = c["dims"]
+    got = run_attn(c, out_dtype, scale=scale).float().cpu().numpy().astype(np.float64).reshape(-1, hq, hd)
+    want, mag = O.tree_attention(c["q"], c["kp"], c["vp"], c["table"], c["ctx"], c["cu"], hq, hk, hd, c["bits"], c["pos"], scale)
+    fp16, out16 = c["q"].dtype == np.float16 and out_dtype == torch.float16, out_dtype == torch.float16
+    err_p = 3 * 64 * E32 * 0.7 + 2.0**-22 + (E16 if fp16 else 2.0**-21)
+    lim = (2 * err_p + (c["max_ctx"] / 16 + 8) * 2.0**-23) * mag + (E16 if out16 else 4 * E32) * np.abs(want) + (TINY16 if out16 else 0)
+    lim = lim + (0 if lost is None else lost)
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    ok = ~np.isnan(want)
+    err = np.abs(got - want)
+    assert np.all((err <= lim)[ok]), (np.max((err / lim)[ok]), np.argwhere(~(err <= lim) & ok)[:4])
+    tree_clean()
+
+
+@pytest.mark.parametrize("hd,T", [(64, 3), (64, 40), (128, 5), (128, 70), (256, 4)])
+@pytest.mark.parametrize("dt", [np.float16, np.float32])
+def test_attn_large_scores(hd, T, dt):
+    """Scores of one large number and small multiples of its last places: +-2^e + d u, u = 2^max(0, e - 21),
+    d in 0 .. 15, exact in fp32.  Up to 2^22 the weights differ by less than e^15; beyond, the scale brings
+    the differences to that, or leaves the rows with the largest (one or several) alone."""
+    r = np.random.default_rng(hd + T)
+    c = attn_case(hd + T, [900, 3, 2000], [T, 2, 1], 4, 2, hd, False, dt=dt)
+    c["vp"] = np.nan_to_num(c["vp"])
+    for e, sign, scale in [(12, 1, 1.0), (20, -1, 0.7), (22, 1, 1.0), (22, -1, 0.9), (25, 1, 0.06), (28, -1, 0.007), (30, 1, 0.0019),
+                           (25, 1, 1.0), (29, -1, 0.3), (30, 1, 0.77), (30, -1, 53.0)]:
+        a = (e + 1) // 2
+        q = np.zeros((c["R"], 4, hd))
+        q[..., 3], q[..., 40] = sign * 2.0**a, 2.0 ** max(0, e - 21)
+        c["q"] = q.reshape(c["R"], -1).astype(dt)
+        c["kp"][:] = 0
+        c["kp"][..., 3] = 2.0 ** (e - a)
+        c["kp"][..., 40] = r.integers(0, 16, c["kp"].shape[:-1])
+        for out in (torch.float16, torch.float32):
+            check_exact_scores(c, out, scale)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attn_scores_that_grow(hd):
+    """The running maximum passes from small scores to ones past 2^22 and on, within one CTA and over several
+    (to 2^27 for 2300 places; 2500 end in an infinite key, whose rows are NaN)."""
+    for ctx, q in (([2300], [9]), ([2500], [9]), ([700] * 80, [1] * 80)):
+        c = attn_case(hd, ctx, q, 2, 1, hd, False)
+        c["vp"] = np.nan_to_num(c["vp"])
+        n = int(c["ctx"][0])
+        c["q"] = np.zeros((c["R"], 2, hd), np.float16)
+        c["q"][:, 0, 1], c["q"][:, 1, 1] = 2.0**12, -(2.0**12)
+        c["q"] = c["q"].reshape(c["R"], -1)
+        c["kp"][:] = 0
+        for b in range(len(ctx)):
+            for j in range(n + q[b]):
+                c["kp"][c["table"][b, j // 16], :, j % 16, 1] = 2.0 ** (j // 100 - 8) if j % 100 == 7 else 0
+        for scale in (1.0, 30.0):
+            check_exact_scores(c, torch.float16, scale)
+            check_exact_scores(c, torch.float32, scale)
