@@ -22,8 +22,10 @@
 // on tcgen05; for one draft of 8 rows over 1021 places 43.7 and 16 us.  So every size goes to
 // tcgen05 where it can.
 //
-// fp32 q (or an output wider than fp16) carries q and the weights as hi + lo fp16 pairs (22 bits),
-// as the decode attention does: two MMAs for one.  No state survives a call, so the workspace
+// fp32 q (or an output wider than fp16) carries q and the weights as hi + lo fp16 pairs, as the decode
+// attention does: two MMAs for one.  A pair has 22 bits down to 2^-14 and no step below 2^-24, so the
+// weights are lifted: the largest is 2^7 .. 2^15 (head_dim 256: 2^15), and what a place loses is 2^-32
+// (2^-40) of it at most.  No state survives a call, so the workspace
 // needs no initial contents and calls on different streams share nothing.
 //
 // Places a row must not see contribute nothing whatever they hold: scores are replaced, not
@@ -50,6 +52,7 @@ constexpr int kRows = 16 * kWarps;              // query rows (t, g) per CTA
 constexpr int kKeys = 64;                       // keys per tile
 constexpr int kMaxChunk = 32768;                // keys per CTA (their page ids are in shared memory)
 constexpr int kMaxWords = 8;
+constexpr float kLift = 15.f;                   // log2 of a row's largest weight
 
 __device__ int g_error;  // a bounded wait gave up (b2d_paged_tree_attn_error)
 
@@ -449,7 +452,8 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
           }
       }
       // running maximum and sum.  Weights are 2^((s - m) c): a product m c of its own would be off by up
-      // to half a step, which is 2^9 for |m c| near 2^33
+      // to half a step, which is 2^9 for |m c| near 2^33.  kLift makes the largest one 2^15: fp16 has
+      // no steps below 2^-24, so the smallest that are kept then are 2^-40 of it
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float m = -INFINITY;
@@ -464,8 +468,8 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
         float part = 0.f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          sc[n][2 * h] = ex2((sc[n][2 * h] - base) * p.scale_log2);
-          sc[n][2 * h + 1] = ex2((sc[n][2 * h + 1] - base) * p.scale_log2);
+          sc[n][2 * h] = ex2(fmaf(sc[n][2 * h] - base, p.scale_log2, kLift));
+          sc[n][2 * h + 1] = ex2(fmaf(sc[n][2 * h + 1] - base, p.scale_log2, kLift));
           part += sc[n][2 * h] + sc[n][2 * h + 1];
         }
         sum[h] = fmaf(sum[h], corr, part);
@@ -475,7 +479,7 @@ __global__ void __launch_bounds__(kThreads) paged_tree_attn_kernel(const __grid_
           o[nd][2 * h + 1] *= corr;
         }
       }
-      // O += P V.  P <= 1 is rounded to fp16 for the product (relative 2^-11, the output's own
+      // O += P V.  P is rounded to fp16 for the product (relative 2^-11, the output's own
       // rounding) unless the result is kept in fp32: then its remainder follows in a second MMA.
 #pragma unroll
       for (int kk = 0; kk < kKeys / 16; ++kk) {

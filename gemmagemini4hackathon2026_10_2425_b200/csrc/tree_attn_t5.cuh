@@ -19,13 +19,14 @@
 // Roles: warps 0-7 softmax (warp w reads TMEM lanes 32 (w % 4) ..), warps 8 and 10 load K and V
 // (TMA), warp 9 issues the MMAs, warp 11 loads the next unit's Q while this one ends.
 //
-// Weights are 2^((s - ref) c), c = scale log2(e), ref a score: a product ref c of its own would be off
+// Weights are 2^((s - ref) c + 7), c = scale log2(e), ref a score: a product ref c of its own would be off
 // by up to half a step, which is 2^9 for |ref c| near 2^33.  The difference is one more operation per
 // pair of scores than a fused s c - ref c.
 //
-// O is rescaled only when a row's maximum has grown by more than 2^8 since the last time (its
-// weights are then up to 256 and still exact to 2^-11 in fp16), which after the first tiles of a
-// unit is almost never; the sum and the weights always use the same reference, so nothing is lost.
+// O is rescaled only when a row's largest weight has grown by more than 2^8 since the last time: it
+// starts at 2^7 and stays below 2^15, inside fp16's range, where what fp16 drops (2^-25) is 2^-32 of
+// it.  After the first tiles of a unit that is almost never; the sum and the weights always use the
+// same reference, so nothing else is lost.
 //
 // Included by tree_attn.cu, whose Params, Span and row helpers it uses.
 #pragma once
@@ -43,6 +44,7 @@ constexpr int kThreads = kSoftmax + 128;    // + K, MMA, V and Q warps
 constexpr int kRegsSoftmax = 224, kRegsOther = 56;
 constexpr int kGroups = 320;                // prefix sums kept, one per `stride` sequences
 constexpr float kSlack = 8.f;               // log2 of the growth that O is rescaled for
+constexpr float kLift = 7.f;                // log2 of the weight of a row's reference
 
 template <int HD, bool MT2, bool X2>
 struct Cfg {
@@ -99,11 +101,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -754,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float base = ref == -INFINITY ? 0.f : ref;  // nothing seen yet: weights 2^-inf
           // weights as fp16 over the scores: relative 2^-11, the output's own rounding; with X2
           // their remainders behind them
-          const uint64_t c2 = two(p.scale_log2, p.scale_log2), b2 = two(-base, -base);
+          const uint64_t c2 = two(p.scale_log2, p.scale_log2), b2 = two(-base, -base), lift = two(kLift, kLift);
           uint64_t acc[2] = {0ull, 0ull};
 #pragma unroll
           for (int h = 0; h < 4; ++h) {
@@ -763,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < 16; ++e) {
               float& x0 = x[32 * h + 2 * e];
               float& x1 = x[32 * h + 2 * e + 1];
-              const float2 z = split(mul2(add2(two(x0, x1), b2), c2));
+              const float2 z = split(fma2(add2(two(x0, x1), b2), c2, lift));
               x0 = ex2(z.x);
               x1 = ex2(z.y);
               acc[e & 1] = add2(acc[e & 1], two(x0, x1));

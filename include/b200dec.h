@@ -399,8 +399,9 @@ B2D_API int b2d_qk_norm_rope_append(const void* qkv, int qkv_dtype, int ldqkv,
  * and NaN included) changes nothing.
  * out [rows, Hq * HD] (F32, F16 or F16X2 with its lo plane at out + rows * ldout; not q itself).
  * fp16 q with an fp16 output multiplies in fp16 with fp32 sums; every other combination carries q
- * and the weights as hi + lo fp16 pairs.  head_dim 64, 128 (tcgen05) or 256 (mma.sync);
- * n_heads / n_kv_heads <= 64.
+ * and the weights as hi + lo fp16 pairs: 22 bits of a q of 2^-14 or more (2^-25 absolute below), and
+ * of a weight 2^-11 (a pair: 2^-22) of itself plus up to 2^-32 of the row's largest weight.
+ * head_dim 64, 128 (tcgen05) or 256 (mma.sync); n_heads / n_kv_heads <= 64.
  * max_q bounds the rows of a sequence and max_ctx every ctx_lens[b] + rows (a sequence beyond
  * max_ctx, and rows beyond max_q, are left as they were).  Block-table entries outside
  * [0, n_blocks) are never dereferenced; their places are hidden.  scale <= 0 means

@@ -94,18 +94,19 @@ def test_attn_window_of_many_tiles(hd):
         check_attn(c, torch.float32, window=window)
 
 
-def check_exact_scores(c, out_dtype, scale, lost=None):
+def check_exact_scores(c, out_dtype, scale, lost=0.0, got=None):
     """Rows whose scores are exact in fp32 and the largest of a row's far weights 2^-64 or nothing.  A weight
     is off by the roundings of z = (s - m) c, |z| <= 64: the difference, the product and c, 2^-24 each (times
     ln 2), and the exponential's 2^-22; then by E16 where it is an fp16 number, 2^-21 as two; `lost` is what
     places of small weight may lose.  Sums over n places: one step per 16."""
     hq, hk, hd = c["dims"]
-    got = run_attn(c, out_dtype, scale=scale).float().cpu().numpy().astype(np.float64).reshape(-1, hq, hd)
+    got = run_attn(c, out_dtype, scale=scale) if got is None else got
+    got = got.float().cpu().numpy().astype(np.float64).reshape(-1, hq, hd)
     want, mag = O.tree_attention(c["q"], c["kp"], c["vp"], c["table"], c["ctx"], c["cu"], hq, hk, hd, c["bits"], c["pos"], scale)
     fp16, out16 = c["q"].dtype == np.float16 and out_dtype == torch.float16, out_dtype == torch.float16
     err_p = 3 * 64 * E32 * 0.7 + 2.0**-22 + (E16 if fp16 else 2.0**-21)
     lim = (2 * err_p + (c["max_ctx"] / 16 + 8) * 2.0**-23) * mag + (E16 if out16 else 4 * E32) * np.abs(want) + (TINY16 if out16 else 0)
-    lim = lim + (0 if lost is None else lost)
+    lim = lim + lost
     np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
     ok = ~np.isnan(want)
     err = np.abs(got - want)
@@ -153,3 +154,33 @@ def test_attn_scores_that_grow(hd):
         for scale in (1.0, 30.0):
             check_exact_scores(c, torch.float16, scale)
             check_exact_scores(c, torch.float32, scale)
+
+
+@pytest.mark.parametrize("hd,T,dt,out", [(64, 1, np.float32, torch.float32), (64, 1, np.float16, torch.float16), (128, 1, np.float32, torch.float16),
+                                         (64, 70, np.float16, torch.float16), (128, 70, np.float16, torch.float16),
+                                         (256, 1, np.float32, torch.float32), (256, 2, np.float16, torch.float16)])
+def test_attn_weak_keys_beside_a_strong_one(hd, T, dt, out):
+    """One key 8 to 21 above thousands of others, whose values alone make the output: their weights are small
+    numbers of fp16 (or of fp16 pairs), none of which may be lost.  A weight is off by 2^-25 at most where
+    fp16 has no smaller step, and the row's largest weight is 2^7 or more: 2^-32 of |v| per place.  More
+    sequences than SMs (of the same pages), so that a CTA sees the strong key and many others."""
+    B, ctx = 160, 8191 if T > 2 else 32767
+    r = np.random.default_rng(hd + T)
+    c = attn_case(hd, [ctx], [T], 2, 1, hd, False, dt=dt)
+    at = lambda j: (c["table"][0, j // 16], slice(None), j % 16)  # noqa: E731
+    c["kp"][:], c["vp"][:] = 0, np.abs(r.standard_normal(c["vp"].shape))
+    c["kp"][..., 1] = r.integers(-8, 9, c["kp"].shape[:-1]) / 16
+    c["kp"][at(100)], c["vp"][at(100)] = 0, 0
+    c["kp"][at(100)][..., 0] = 16
+    strong = np.linspace(8, 21, B * T * 2).reshape(-1, 2)
+    q = np.zeros((B * T, 2, hd))
+    q[..., 0], q[..., 1] = strong * hd**0.5 / 16, hd**0.5
+    few = [0, B // 2, B - 1]
+    for name, n in (("many", B), ("few", len(few))):
+        c[name] = dict(c, table=np.repeat(c["table"], n, 0), ctx=np.repeat(c["ctx"], n), cu=(np.arange(n + 1) * T).astype(np.int32),
+                       pos=np.tile(c["pos"], n), R=n * T)
+    c["many"]["q"] = q.reshape(B * T, -1).astype(dt)
+    c["few"]["q"] = np.concatenate([c["many"]["q"][b * T : (b + 1) * T] for b in few])
+    got = run_attn(c["many"], out)
+    got = torch.cat([got[b * T : (b + 1) * T] for b in few])
+    check_exact_scores(c["few"], out, 0.0, lost=c["vp"].astype(np.float64).sum((0, 2)).max() * 2.0**-32, got=got)
