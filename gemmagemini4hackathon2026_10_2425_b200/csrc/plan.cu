@@ -248,7 +248,16 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const Params p) {
   }
   for (int b = tid >> 5; b < p.batch; b += kThreads / 32) {
     const Req r = req[b];
-    if (r.have < 0 || r.off == kRefused) continue;
+    if (r.have < 0) continue;
+    if (r.off == kRefused) {
+      // entries that an earlier owner of the row left behind are not this request's: its rows would
+      // attend to them
+      if (r.ctx < 0) continue;
+      const long long blocks = ((long long)r.ctx + (req[b + 1].row - r.row) + 15) / 16;
+      const int end = (int)min(blocks, (long long)p.max_blocks);
+      for (int j = r.have + rank * 32 + lane; j < end; j += ranks * 32) p.table[(size_t)b * p.max_blocks + j] = -1;
+      continue;
+    }
     const int need = (r.ctx + req[b + 1].row - r.row + 15) / 16 - r.have;
 #pragma unroll 4
     for (int j = rank * 32 + lane; j < need; j += ranks * 32)

@@ -722,7 +722,9 @@ def paged_plan(
 ) -> PagedPlan:
     """Pages, slots, positions and tree masks of a step that adds q_lens[b] rows to request b (a
     negative number ends it and gives its pages back); block_table and free_pages are updated in
-    place, n_pages and n_free if `out` holds them.  See include/b200dec.h b2d_paged_plan.  ctx_lens,
+    place, n_pages and n_free if `out` holds them.  A request with status != PLAN_OK was not served:
+    its rows exist without slots, and what a step computes for them is to be dropped.  See
+    include/b200dec.h b2d_paged_plan.  ctx_lens,
     q_lens, n_pages int32 [B]; block_table int32 [B, max_blocks]; free_pages int32 [capacity]; n_free
     int32 [1]; parents int32 [max_tokens] with mask_words (<= 8) words of 32 nodes per row."""
     d, B = _on_gpu(ctx_lens), ctx_lens.numel()

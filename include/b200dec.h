@@ -350,7 +350,11 @@ enum b2d_plan_status {
  *   q_lens[b] < 0: the request ended.  Its pages are pushed onto the stack, before any are popped;
  *     its block-table row keeps its (now meaningless) entries.
  * A request that cannot be served keeps its pages and gets status[b] != 0; its rows exist with
- * slots -1 (b2d_qk_norm_rope_append then stores nothing).  The pages asked for by a refused
+ * slots -1 (b2d_qk_norm_rope_append then stores nothing), and the block-table entries behind its
+ * pages that they would need become -1, so that b2d_paged_tree_attn does not follow what an earlier
+ * request left there.  What the step computes for these rows means nothing and has to be dropped:
+ * their own k and v are not in the cache, and the end of the request's last page holds whatever
+ * was there.  The pages asked for by a refused
  * request still count against the requests after it, so whether one is served depends on those
  * before it only.  Outputs: cu_q[batch + 1] (first rows), slots (page * 16 + place in the page,
  * or -1) and positions per row, n_pages_out[batch] and n_free_out[1] (may be n_pages and n_free),

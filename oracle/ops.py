@@ -374,6 +374,8 @@ def paged_plan(ctx, q, table, n_pages, stack, n_free, max_tokens: int, parents=N
         r0, r1 = cu[-1], min(end, max_tokens)
         cu.append(r1)
         k = r1 - r0
+        if st != PLAN_OK and c >= 0:
+            table[b, have : -(-(c + k) // PAGE_TOKENS)] = -1
         positions[r0:r1] = c + np.arange(k)
         if words and k:
             bits, depth = tree_bits(parents[r0:r1])

@@ -6,8 +6,11 @@ import numpy as np
 import pytest
 import torch
 
+from gemmagemini4hackathon2026_10_2425_b200 import _lib, ops
 from oracle import ops as O
-from test_draft_step_gpu import DEV, E16, E32, TINY16, attn_case, check_attn, check_score, run_attn, tree_clean
+from test_draft_step_gpu import (
+    DEV, E16, E32, TINY16, attn_bound, attn_case, check_attn, check_plan, check_score, gpu, i32, run_attn, run_plan, same, tree_clean
+)
 
 pytestmark = pytest.mark.gpu
 
@@ -184,3 +187,45 @@ def test_attn_weak_keys_beside_a_strong_one(hd, T, dt, out):
     got = run_attn(c["many"], out)
     got = torch.cat([got[b * T : (b + 1) * T] for b in few])
     check_exact_scores(c["few"], out, 0.0, lost=c["vp"].astype(np.float64).sum((0, 2)).max() * 2.0**-32, got=got)
+
+
+# -- refused requests -----------------------------------------------------------------------------
+
+
+def test_plan_refused_rows_have_no_stale_pages():
+    """Table rows that still name an earlier request's pages: a refused request's places there have none,
+    whatever it was refused for; served and ended requests keep theirs."""
+    stale = np.arange(50, 50 + 7 * 8, dtype=np.int32).reshape(7, 8)
+    c = dict(ctx=np.array([20, 100, -3, 5, 10, 0, 3]), q=np.array([30, 60, 2, 40, 1, -1, 90]), table=stale, n_pages=np.array([2, 3, 0, 1, 1, 0, 0]),
+             stack=np.arange(200, 230, dtype=np.int32), n_free=1, R=140, parents=np.full(140, -1, np.int32), words=1)
+    w = check_plan(c)
+    assert w["status"].tolist() == [_lib.PLAN_PAGES, _lib.PLAN_TABLE, _lib.PLAN_TABLE, _lib.PLAN_TREE, 0, 0, _lib.PLAN_ROWS]
+    assert w["table"][0].tolist() == [50, 51, -1, -1, 54, 55, 56, 57] and w["table"][1, 3:].tolist() == [-1] * 5
+    assert w["table"][3, 1:4].tolist() == [-1, -1, 77] and w["table"][6, 0] == -1
+    for b in (2, 4, 5):
+        assert w["table"][b].tolist() == stale[b].tolist()
+    c["words"], c["parents"] = 0, None
+    check_plan(c)
+
+
+def test_refused_rows_see_no_other_request():
+    """A slot whose table row still holds an ended request's pages, given to a request that is refused: its
+    rows attend to nothing there (the pages hold NaN), the served request beside it is untouched."""
+    hq, hk, hd = 4, 2, 64
+    table = np.array([[3, 4, 5, 6], [0, 1, -1, -1]], np.int32)
+    c = dict(ctx=np.array([0, 20]), q=np.array([40, 5]), table=table, n_pages=np.array([0, 2]), stack=np.zeros(4, np.int32), n_free=0, R=45,
+             parents=None, words=0)
+    plan, dev = run_plan(c)
+    same(plan.status, [_lib.PLAN_PAGES, 0])
+    a = attn_case(5, [20], [5], hq, hk, hd, False)
+    kp = torch.full((8, hk, 16, hd), float("nan"), dtype=torch.float16, device=DEV)
+    vp = kp.clone()
+    for src, dst in ((a["kp"], kp), (a["vp"], vp)):
+        dst[:2] = gpu(src)[gpu(a["table"][0]).long()]
+    q = torch.randn(45, hq * hd, device=DEV)
+    q[40:] = gpu(a["q"])
+    got = ops.paged_tree_attn(q, kp, vp, dev["table"], i32(c["ctx"]), plan.cu_q, hq, hk, hd, 40, 64)
+    assert got[:40].eq(0).all()
+    a["q"] = a["q"].astype(np.float32)
+    want, mag = O.tree_attention(a["q"], a["kp"], a["vp"], a["table"], a["ctx"], a["cu"], hq, hk, hd)
+    assert np.all(np.abs(got[40:].cpu().numpy().reshape(want.shape) - want) <= attn_bound(a, want, mag, False, False, 0))
