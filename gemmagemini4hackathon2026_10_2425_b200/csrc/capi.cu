@@ -96,7 +96,7 @@ const char* b2d_status_string(int status) {
     case B2D_ERR_NULL: return "a required pointer is NULL";
     case B2D_ERR_SHAPE: return "sizes out of range or not supported";
     case B2D_ERR_ALIGN: return "pointer or row stride not 16-byte aligned";
-    case B2D_ERR_UNSUPPORTED: return "dtype / epilogue / head_dim combination not supported";
+    case B2D_ERR_UNSUPPORTED: return "dtype / epilogue / head_dim combination or overlap of buffers not supported";
     case B2D_ERR_WORKSPACE: return "workspace missing or too small";
     case B2D_ERR_CUDA: return "CUDA runtime error";
     case B2D_ERR_NCCL: return "NCCL error";

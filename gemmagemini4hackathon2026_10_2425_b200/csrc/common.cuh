@@ -32,6 +32,21 @@ inline int launch_status() {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Do any of two buffers' rows share memory?  (rows * ld bytes apart each, of width bytes; rows of one
+// may lie between those of the other.)
+inline bool rows_overlap(const void* a, long long rows_a, long long ld_a, long long width_a, const void* b,
+                         long long rows_b, long long ld_b, long long width_b) {
+  const long long a0 = (long long)reinterpret_cast<uintptr_t>(a), b0 = (long long)reinterpret_cast<uintptr_t>(b);
+  if (a0 + (rows_a - 1) * ld_a + width_a <= b0 || b0 + (rows_b - 1) * ld_b + width_b <= a0) return false;
+  for (long long i = 0, j = 0; i < rows_a && j < rows_b;) {
+    const long long x = a0 + i * ld_a, y = b0 + j * ld_b;
+    if (x + width_a <= y) ++i;
+    else if (y + width_b <= x) ++j;
+    else return true;
+  }
+  return false;
+}
+
 int num_sms();  // cached per device
 
 #define B2D_TRY(expr)              \

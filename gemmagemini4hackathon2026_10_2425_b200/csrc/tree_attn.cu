@@ -707,6 +707,12 @@ int paged_tree_attn(const void* q, int q_dtype, int ldq, const uint16_t* k_pages
       paged_tree_attn_workspace_bytes(batch, rows, n_heads, n_kv_heads, head_dim, max_q, max_ctx);
   if (need && (!workspace || workspace_bytes < need)) return B2D_ERR_WORKSPACE;
   if (!aligned16(workspace)) return B2D_ERR_ALIGN;
+  // rows of q are read while rows of out are written
+  const int qe = q_dtype == B2D_F16 ? 2 : 4, oe = out_dtype == B2D_F32 ? 4 : 2;
+  const long long width = (long long)n_heads * head_dim;
+  if (rows_overlap(q, rows, (long long)ldq * qe, width * qe, out, out_dtype == B2D_F16X2 ? 2ll * rows : rows,
+                   (long long)ldout * oe, width * oe))
+    return B2D_ERR_UNSUPPORTED;
   tree::Params p = {};
   B2D_TRY(make_tmap_f16(&p.tmK, k_pages, prows, head_dim, head_dim, 16));
   p.q = q;

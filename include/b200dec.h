@@ -50,7 +50,7 @@ enum b2d_status {
   B2D_ERR_NULL = 1,        /* a required pointer is NULL */
   B2D_ERR_SHAPE = 2,       /* sizes out of range or not supported by the kernel */
   B2D_ERR_ALIGN = 3,       /* pointer or row stride not 16-byte aligned */
-  B2D_ERR_UNSUPPORTED = 4, /* dtype / epilogue / head_dim combination not built */
+  B2D_ERR_UNSUPPORTED = 4, /* dtype / epilogue / head_dim combination not built, or buffers that overlap */
   B2D_ERR_WORKSPACE = 5,   /* workspace missing or smaller than the *_workspace_bytes query */
   B2D_ERR_CUDA = 6,        /* a CUDA runtime call failed (see b2d_last_cuda_error) */
   B2D_ERR_NCCL = 7,        /* an NCCL call failed */
@@ -401,7 +401,8 @@ B2D_API int b2d_qk_norm_rope_append(const void* qkv, int qkv_dtype, int ldqkv,
  * rows have positions[row] (required then; b2d_paged_plan's: row i's is held to ctx_lens[b] ..
  * ctx_lens[b] + i).  A row that sees nothing gives zeros.  What a hidden place holds (infinities
  * and NaN included) changes nothing.
- * out [rows, Hq * HD] (F32, F16 or F16X2 with its lo plane at out + rows * ldout; not q itself).
+ * out [rows, Hq * HD] (F32, F16 or F16X2 with its lo plane at out + rows * ldout).  Rows
+ * of out may lie between rows of q, but share no memory with any (B2D_ERR_UNSUPPORTED).
  * fp16 q with an fp16 output multiplies in fp16 with fp32 sums; every other combination carries q
  * and the weights as hi + lo fp16 pairs: 22 bits of a q of 2^-14 or more (2^-25 absolute below), and
  * of a weight 2^-11 (a pair: 2^-22) of itself plus up to 2^-32 of the row's largest weight.

@@ -229,3 +229,19 @@ def test_refused_rows_see_no_other_request():
     a["q"] = a["q"].astype(np.float32)
     want, mag = O.tree_attention(a["q"], a["kp"], a["vp"], a["table"], a["ctx"], a["cu"], hq, hk, hd)
     assert np.all(np.abs(got[40:].cpu().numpy().reshape(want.shape) - want) <= attn_bound(a, want, mag, False, False, 0))
+
+
+# -- buffers that overlap, or lie close together ----------------------------------------------------
+
+
+def test_attn_rows_of_out_between_rows_of_q():
+    hq, hk, hd = 8, 2, 64
+    c = attn_case(10, [50, 20], [6, 2], hq, hk, hd, True)
+    want = run_attn(c, torch.float16)
+    wide = torch.zeros(c["R"], 2 * hq * hd, dtype=torch.float16, device=DEV)
+    wide[:, : hq * hd] = gpu(c["q"])
+    run_attn(c, q=wide[:, : hq * hd], out=wide[:, hq * hd :])
+    assert torch.equal(wide[:, hq * hd :], want) and torch.equal(wide[:, : hq * hd], gpu(c["q"]))
+    for out in (wide[:, : hq * hd], wide[:, 64 : hq * hd + 64], wide[:, hq * hd - 8 : -8]):
+        with pytest.raises(ValueError, match="overlap"):
+            run_attn(c, q=wide[:, : hq * hd], out=out)
