@@ -190,6 +190,13 @@ int qk_norm_rope_append(const void* qkv, int qkv_dtype, int ldqkv, const float* 
       !aligned16(q_gamma) || !aligned16(k_gamma) || ldqkv % (qkv_dtype == B2D_F16 ? 8 : 4) ||
       ldq % (q_dtype == B2D_F16 ? 8 : 4))
     return B2D_ERR_ALIGN;
+  // a value may be written where it was read (in place), but nowhere else in qkv: other lanes and
+  // rows read there at the same time
+  const int xe = qkv_dtype == B2D_F16 ? 2 : 4, oe = q_dtype == B2D_F16 ? 2 : 4;
+  const bool in_place = q_out == qkv && q_dtype == qkv_dtype && (ldq == ldqkv || rows == 1);
+  if (!in_place && rows_overlap(qkv, rows, (long long)ldqkv * xe, (long long)(n_heads + 2 * n_kv_heads) * head_dim * xe,
+                                q_out, rows, (long long)ldq * oe, (long long)n_heads * head_dim * oe))
+    return B2D_ERR_UNSUPPORTED;
   const qka::Params p = {qkv,      ldqkv,   q_gamma,  k_gamma, eps,
                          v_norm,   positions, slots,  n_rows,  inv_freq,
                          q_out,    ldq,     k_pages,  v_pages, (long long)n_blocks * 16,

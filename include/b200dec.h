@@ -378,7 +378,8 @@ B2D_API int b2d_paged_plan(const int* ctx_lens, const int* q_lens, const int* pa
  * head: x * rsqrt(mean(x^2) + eps) * gamma with q_gamma / k_gamma [HD] (NULL: no norm), then the
  * rotation of the pairs (i, i + HD/2) by positions[row] * inv_freq[i] (a zero inv_freq leaves its
  * pair alone).  v is normalized without a weight if v_norm.  q goes to q_out (F32 or F16, row
- * stride ldq; qkv itself with ldq = ldqkv is allowed for equal types), k and v rounded to fp16
+ * stride ldq; qkv itself with ldq = ldqkv is allowed for equal types, any other overlap of their
+ * rows is not: B2D_ERR_UNSUPPORTED), k and v rounded to fp16
  * to slot slots[row] of the pages.  Rows with positions[row] < 0, and rows from *n_rows on (a
  * device int, e.g. cu_q + batch; NULL: all rows), are skipped; slots outside [0, n_blocks * 16)
  * (or slots NULL) store nothing.  Two rows with the same slot leave either's values there.

@@ -9,7 +9,8 @@ import torch
 from gemmagemini4hackathon2026_10_2425_b200 import _lib, ops
 from oracle import ops as O
 from test_draft_step_gpu import (
-    DEV, E16, E32, TINY16, attn_bound, attn_case, check_attn, check_plan, check_score, gpu, i32, run_attn, run_plan, same, tree_clean
+    DEV, E16, E32, TINY16, attn_bound, attn_case, check_attn, check_plan, check_qk, check_score, gpu, i32, qk_case, run_attn,
+    run_plan, same, tree_clean,
 )
 
 pytestmark = pytest.mark.gpu
@@ -232,6 +233,21 @@ def test_refused_rows_see_no_other_request():
 
 
 # -- buffers that overlap, or lie close together ----------------------------------------------------
+
+
+def test_qk_rows_of_q_out_between_rows_of_qkv():
+    hq, hk, hd, R = 6, 2, 64, 21
+    c, n = qk_case(2, R, hq, hk, hd, np.float16), (hq + 2 * hk) * hd
+    wide = torch.zeros(R, n + hq * hd, dtype=torch.float16, device=DEV)
+    wide[:, :n] = gpu(c["x"])
+    check_qk(c, torch.float16, x_dev=wide[:, :n], q_out=wide[:, n:])
+    same(wide[:, :n], c["x"])
+    for q_out in (wide[:, 8 : hq * hd + 8], wide[:, n - 8 : -8]):
+        with pytest.raises(ValueError, match="overlap"):
+            check_qk(c, torch.float16, x_dev=wide[:, :n], q_out=q_out)
+    one = gpu(c["x"])[:1].contiguous()  # a single row in place
+    c.update({k: c[k][:1] for k in ("x", "pos", "slots")})
+    check_qk(c, torch.float16, x_dev=one, q_out=one[:, : hq * hd])
 
 
 def test_attn_rows_of_out_between_rows_of_q():

@@ -4,7 +4,7 @@ CUDA call (the addresses are never dereferenced)."""
 import pytest
 
 from gemmagemini4hackathon2026_10_2425_b200 import _lib
-from test_draft_step import P, attn_args
+from test_draft_step import P, attn_args, qk_args
 
 WS = dict(ws=P, wsb=1 << 40)
 
@@ -20,3 +20,14 @@ WS = dict(ws=P, wsb=1 << 40)
 ])
 def test_attn_out_shares_memory_with_q(kw):
     assert _lib.lib().b2d_paged_tree_attn(*attn_args(**WS, **kw)) == _lib.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("kw", [
+    dict(ldq=64),  # qkv itself, its rows closer together
+    dict(odt=1, ldq=384),  # another type
+    dict(out=P + 256, ldq=192),  # k's place
+    dict(out=P + 3 * 768 - 16, ldq=192),  # the last row's v
+    dict(qkv=P + 2 * 768 + 256 - 16, ldq=192),  # out's last row
+])
+def test_qk_out_shares_memory_with_qkv(kw):
+    assert _lib.lib().b2d_qk_norm_rope_append(*qk_args(rows=3, **kw)) == _lib.ERR_UNSUPPORTED
