@@ -726,7 +726,8 @@ def paged_plan(
     its rows exist without slots, and what a step computes for them is to be dropped.  See
     include/b200dec.h b2d_paged_plan.  ctx_lens,
     q_lens, n_pages int32 [B]; block_table int32 [B, max_blocks]; free_pages int32 [capacity]; n_free
-    int32 [1]; parents int32 [max_tokens] with mask_words (<= 8) words of 32 nodes per row."""
+    int32 [1]; parents int32 [max_tokens] with mask_words (<= 8) words of 32 nodes per row.  A batch of
+    no requests gives no rows; max_tokens is at least 1."""
     d, B = _on_gpu(ctx_lens), ctx_lens.numel()
     _check("ctx_lens", ctx_lens, _I32, d, (B,))
     _check("q_lens", q_lens, _I32, d, (B,))
@@ -737,6 +738,8 @@ def paged_plan(
     _check("parents", parents, _I32, d, (max_tokens,))
     if (parents is None) != (mask_words == 0):
         raise ValueError("parents and mask_words go together")
+    if max_tokens < 1:
+        raise ValueError("max_tokens must be at least 1 (a step without rows has buffers too)")
     if out is None:
         new = ctx_lens.new_empty
         out = PagedPlan(
@@ -759,6 +762,10 @@ def paged_plan(
             if out.mask is None:
                 raise ValueError("out.mask is missing")
             _check("out.mask", out.mask, _I32, d, (max_tokens, mask_words))
+    if B == 0:  # no requests: no rows, and the free stack as it was
+        out.cu_q.zero_()
+        torch.clamp(n_free, 0, free_pages.numel(), out=out.n_free)
+        return out
     _call_on(
         d,
         "b2d_paged_plan",
@@ -900,7 +907,7 @@ def paged_tree_attn(
     _check("cu_q", cu_q, _I32, d, (B + 1,))
     _check("mask", mask, _I32, d, (R, *(() if mask is None else mask.shape[1:2])))
     _check("positions", positions, _I32, d, (R,))
-    if R == 0:
+    if R == 0 or B == 0:  # no row belongs to a sequence
         return out
     nbytes = tree_attn_workspace_bytes(B, R, n_heads, n_kv_heads, head_dim, max_q, max_ctx)
     if workspace is None:

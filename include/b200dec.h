@@ -363,7 +363,7 @@ enum b2d_plan_status {
  * the request, of the row a drafted token follows, less than its own; -1, or anything else, the
  * last cached token) they are ctx_lens[b] + depth, and mask[row][mask_words] (mask_words <= 8)
  * has bit j set if row j of the request is the row itself or an ancestor of it.
- * max_tokens <= 2^24 is the size of the row arrays, free_capacity that of free_pages (pages
+ * max_tokens, 1 .. 2^24, is the size of the row arrays, free_capacity that of free_pages (pages
  * pushed past it are lost), max_blocks <= 2^17. */
 B2D_API int b2d_paged_plan(const int* ctx_lens, const int* q_lens, const int* parents,
                            int* block_table, int max_blocks, const int* n_pages, int* free_pages,

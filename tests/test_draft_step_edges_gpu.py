@@ -261,3 +261,26 @@ def test_attn_rows_of_out_between_rows_of_q():
     for out in (wide[:, : hq * hd], wide[:, 64 : hq * hd + 64], wide[:, hq * hd - 8 : -8]):
         with pytest.raises(ValueError, match="overlap"):
             run_attn(c, q=wide[:, : hq * hd], out=out)
+
+
+# -- nothing to do ------------------------------------------------------------------------------------
+
+
+def test_empty_batches_and_rows():
+    """No requests, or no rows: every call returns, outputs of the sizes asked for, buffers untouched."""
+    z = lambda *n, t=torch.int32: torch.zeros(*n, dtype=t, device=DEV)  # noqa: E731
+    kp, vp = z(3, 2, 16, 64, t=torch.float16), z(3, 2, 16, 64, t=torch.float16)
+    stack, n_free = i32([4, 5, 6]), i32([2])
+    p = ops.paged_plan(z(0), z(0), z(0, 7), z(0), stack, n_free, 5)
+    assert p.cu_q.tolist() == [0] and p.n_free.tolist() == [2] and p.status.numel() == 0 and p.slots.shape == (5,)
+    p = ops.paged_plan(z(0), z(0), z(0, 7), z(0), stack, n_free, 5, out=ops.PagedPlan(p.cu_q.fill_(9), p.slots, p.positions, None, z(0), z(0), n_free))
+    assert p.cu_q.tolist() == [0] and n_free.tolist() == [2] and stack.tolist() == [4, 5, 6]
+    with pytest.raises(ValueError, match="max_tokens"):
+        ops.paged_plan(z(2), z(2), z(2, 7), z(2), stack, n_free, 0)
+    out = torch.full((5, 256), 3.0, device=DEV)
+    for rows in (5, 0):
+        got = ops.paged_tree_attn(z(rows, 256, t=torch.float32), kp, vp, z(0, 7), z(0), z(1), 4, 2, 64, 2, 32, out=out[:rows])
+        assert got.shape == (rows, 256)
+    assert out.eq(3).all()
+    assert ops.qk_norm_rope_append(z(0, 512, t=torch.float32), z(0), z(0, t=torch.int64), z(32, t=torch.float32), kp, vp, 4, 2, 64).shape == (0, 256)
+    assert ops.token_logprobs(z(0, 50, t=torch.float32), z(0), 3).top_ids.shape == (0, 3)
