@@ -658,8 +658,19 @@ def _on_gpu(t: torch.Tensor) -> int:
 
 
 def _ld(t: torch.Tensor) -> int:
-    """Row stride of a [rows, n] tensor whose rows do not overlap."""
-    return max(t.stride(0), t.shape[1])
+    """Row stride of a [rows, n] tensor whose rows do not overlap (a single row's says nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _two_dims(name: str, t: torch.Tensor) -> None:
+    if t.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions, not {t.dim()}")
+
+
+def _fits32(*args: int) -> None:
+    """ctypes cuts an int to its low 32 bits without a word."""
+    if max(args) > 0x7FFFFFFF or min(args) < -0x80000000:
+        raise ValueError(f"an integer argument or row stride does not fit 32 bits: {max(args, key=abs)}")
 
 
 # the current stream's handle without a Stream object around it (1.2 us less per call), where torch has it
@@ -729,9 +740,11 @@ def paged_plan(
     int32 [1]; parents int32 [max_tokens] with mask_words (<= 8) words of 32 nodes per row.  A batch of
     no requests gives no rows; max_tokens is at least 1."""
     d, B = _on_gpu(ctx_lens), ctx_lens.numel()
+    _two_dims("block_table", block_table)
+    _fits32(max_tokens, mask_words)
     _check("ctx_lens", ctx_lens, _I32, d, (B,))
     _check("q_lens", q_lens, _I32, d, (B,))
-    _check("block_table", block_table, _I32, d, (B, *block_table.shape[1:2]))
+    _check("block_table", block_table, _I32, d, (B, block_table.shape[1]))
     _check("n_pages", n_pages, _I32, d, (B,))
     _check("free_pages", free_pages, _I32, d, (free_pages.numel(),))
     _check("n_free", n_free, _I32, d, (1,))
@@ -820,6 +833,7 @@ def qk_norm_rope_append(
     v to their slots, for rows of qkv [R, (Hq + 2 Hkv) * HD]; returns the rotated q [R, Hq * HD].
     See include/b200dec.h b2d_qk_norm_rope_append.  positions int32 [R], slots int64 [R] and n_rows
     (int32 [1], optional: rows in use) as paged_plan returns them."""
+    _two_dims("qkv", qkv)
     d, R, nq = _on_gpu(qkv), qkv.shape[0], n_heads * head_dim
     _check("qkv", qkv, _FLOATS, d, (R, (n_heads + 2 * n_kv_heads) * head_dim), rows=True)
     if q_out is None:
@@ -834,6 +848,7 @@ def qk_norm_rope_append(
     _check_pages(k_pages, v_pages, n_kv_heads, head_dim, d)
     if R == 0:
         return q_out
+    _fits32(_ld(qkv), _ld(q_out), n_heads, n_kv_heads, head_dim, R, k_pages.shape[0])
     _call_on(
         d,
         "b2d_qk_norm_rope_append",
@@ -892,6 +907,10 @@ def paged_tree_attn(
     HD] is rotated, the rows' k and v are in the cache.  See include/b200dec.h b2d_paged_tree_attn;
     `out` may be fp16 [2, R, Hq * HD]: the output as B2D_F16X2 hi + lo planes.  The workspace (any
     contents) is allocated from torch's caching allocator unless given."""
+    _two_dims("q", q)
+    _two_dims("block_table", block_table)
+    if mask is not None:
+        _two_dims("mask", mask)
     d, R, nq, B = _on_gpu(q), q.shape[0], n_heads * head_dim, ctx_lens.numel()
     _check("q", q, _FLOATS, d, (R, nq), rows=True)
     if out is None:
@@ -903,12 +922,14 @@ def paged_tree_attn(
         _check("out", out, _FLOATS, d, (R, nq), rows=True)
     _check_pages(k_pages, v_pages, n_kv_heads, head_dim, d)
     _check("ctx_lens", ctx_lens, _I32, d, (B,))
-    _check("block_table", block_table, _I32, d, (B, *block_table.shape[1:2]))
+    _check("block_table", block_table, _I32, d, (B, block_table.shape[1]))
     _check("cu_q", cu_q, _I32, d, (B + 1,))
-    _check("mask", mask, _I32, d, (R, *(() if mask is None else mask.shape[1:2])))
+    _check("mask", mask, _I32, d, None if mask is None else (R, mask.shape[1]))
     _check("positions", positions, _I32, d, (R,))
     if R == 0 or B == 0:  # no row belongs to a sequence
         return out
+    ldout = nq if x2 else _ld(out)
+    _fits32(_ld(q), ldout, n_heads, n_kv_heads, head_dim, R, k_pages.shape[0], max_q, max_ctx, window)
     nbytes = tree_attn_workspace_bytes(B, R, n_heads, n_kv_heads, head_dim, max_q, max_ctx)
     if workspace is None:
         if nbytes:
@@ -942,7 +963,7 @@ def paged_tree_attn(
         window,
         out.data_ptr(),
         _lib.F16X2 if x2 else _DT[out.dtype],
-        nq if x2 else _ld(out),
+        ldout,
         _ptr(workspace),
         0 if workspace is None else workspace.numel(),
     )
@@ -1004,6 +1025,7 @@ def token_logprobs(
             _check("out.top_logprobs", out.top_logprobs, _F32, d, (R, top_k))
     if R == 0:
         return out
+    _fits32(R, V, top_k)
     _call_on(
         d,
         "b2d_token_logprobs",

@@ -284,3 +284,57 @@ def test_empty_batches_and_rows():
     assert out.eq(3).all()
     assert ops.qk_norm_rope_append(z(0, 512, t=torch.float32), z(0), z(0, t=torch.int64), z(32, t=torch.float32), kp, vp, 4, 2, 64).shape == (0, 256)
     assert ops.token_logprobs(z(0, 50, t=torch.float32), z(0), 3).top_ids.shape == (0, 3)
+
+
+# -- arguments that the C interface cannot carry -----------------------------------------------------------
+
+
+def test_integers_and_strides_past_32_bits_are_refused():
+    """ctypes keeps the low 32 bits of an int: window = 2^32 + 5 would have been 5, a row stride another row."""
+    c = attn_case(1, [20], [3], 4, 2, 64, True)
+    for kw in (dict(window=2**32 + 5), dict(max_q=2**32 + 3), dict(max_ctx=2**32 + 23)):
+        with pytest.raises(ValueError, match="32 bits"):
+            run_attn(c, **kw)
+    x = logits(2, 100)
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.token_logprobs(x, None, 2**32 + 3)
+    z = lambda *n: torch.zeros(*n, dtype=torch.int32, device=DEV)  # noqa: E731
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.paged_plan(z(1), z(1), z(1, 2), z(1), z(4), z(1), 2, parents=z(2), mask_words=2**32 + 1)
+    wide = torch.empty(2**32 + 8192, dtype=torch.float16, device=DEV)
+    far = wide.as_strided((2, 256), (2**32 + 4096, 1))
+    far.copy_(gpu(attn_case(2, [9], [2], 4, 2, 64, False)["q"]))
+    a = attn_case(2, [9], [2], 4, 2, 64, False)
+    with pytest.raises(ValueError, match="32 bits"):
+        run_attn(a, q=far)
+    with pytest.raises(ValueError, match="32 bits"):
+        run_attn(a, out=far)
+    q = qk_case(3, 2, 2, 1, 64, np.float16)
+    for kw in (dict(x_dev=far), dict(x_dev=gpu(q["x"]), q_out=far[:, :128])):
+        with pytest.raises(ValueError, match="32 bits"):
+            check_qk(q, torch.float16, **kw)
+    check_score(far, np.zeros((2, 1), int), 3)  # this one takes 64 bits
+
+
+def test_a_single_row_of_any_stride():
+    """One row's stride says nothing, whatever it is."""
+    a = attn_case(2, [9], [1], 4, 2, 64, False)
+    row = gpu(a["q"]).as_strided((1, 256), (3, 1))
+    assert torch.equal(run_attn(a, q=row), run_attn(a))
+    q = qk_case(3, 1, 2, 1, 64, np.float16)
+    check_qk(q, torch.float16, x_dev=gpu(q["x"]).as_strided((1, 256), (5, 1)))
+
+
+def test_tables_and_masks_without_two_dimensions_are_refused():
+    c = attn_case(1, [20], [3], 4, 2, 64, True)
+    z = lambda *n: torch.zeros(*n, dtype=torch.int32, device=DEV)  # noqa: E731
+    with pytest.raises(ValueError):
+        run_attn(dict(c, table=c["table"][:, 0]))
+    with pytest.raises(ValueError):
+        run_attn(c, mask=gpu(c["mask"])[:, 0].contiguous())
+    with pytest.raises(ValueError):
+        run_attn(c, q=gpu(c["q"])[0])
+    with pytest.raises(ValueError):
+        ops.paged_plan(z(3), z(3), z(3), z(3), z(4), z(1), 2)
+    with pytest.raises(ValueError):
+        ops.qk_norm_rope_append(torch.zeros((), device=DEV), z(1), z(1).long(), torch.zeros(32, device=DEV), gpu(c["kp"]), gpu(c["vp"]), 4, 2, 64)
