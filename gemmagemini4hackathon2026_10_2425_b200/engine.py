@@ -247,17 +247,26 @@ class DecodeEngine:
 
     # -- step -------------------------------------------------------------------------------
 
-    def _take(self, *tensors: torch.Tensor | None) -> None:
+    def _take(self, *tensors: torch.Tensor | None) -> torch.cuda.Stream | None:
         """Order self.stream after the caller's current stream, which made the tensors, and keep their
         memory from being handed out again while a step still reads it (a caller that makes new ones
-        for every step runs ahead of the GPU).  Nothing to do for a caller on self.stream."""
+        for every step runs ahead of the GPU).  Nothing to do for a caller on self.stream.  The caller's
+        stream is returned if it is being captured: self.stream is then part of the capture, and
+        _give() has to join it back."""
         cur = torch.cuda.current_stream(self.device)
         if cur == self.stream:
-            return
+            return None
+        with torch.cuda.device(self.device):
+            capturing = torch.cuda.is_current_stream_capturing()
         self.stream.wait_stream(cur)
         for t in tensors:
             if t is not None:
                 t.record_stream(self.stream)
+        return cur if capturing else None
+
+    def _give(self, captured: torch.cuda.Stream | None) -> None:
+        if captured is not None:
+            captured.wait_stream(self.stream)
 
     def step(
         self,
@@ -269,26 +278,30 @@ class DecodeEngine:
         use_graph: bool = True,
     ) -> torch.Tensor:
         """Enqueue one decode step on self.stream (no host sync).  tokens/ctx_lens/next_tokens
-        int32 [B]; block_table int32 [B, max_blocks]; logits (optional) fp32 [B, lm_rows]."""
+        int32 [B]; block_table int32 [B, max_blocks]; logits (optional) fp32 [B, lm_rows].  If the
+        caller's stream is being captured, the step becomes part of that capture."""
         B = tokens.numel()
         for t in (tokens, ctx_lens, block_table, next_tokens):
             if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
                 raise ValueError("tokens, ctx_lens, block_table, next_tokens: contiguous CUDA int32")
         if block_table.shape != (B, self.max_blocks):
             raise ValueError(f"block_table must be [{B}, {self.max_blocks}]")
-        self._take(tokens, ctx_lens, block_table, next_tokens, logits)
-        call(
-            "b2d_decoder_step",
-            self._h,
-            tokens.data_ptr(),
-            ctx_lens.data_ptr(),
-            block_table.data_ptr(),
-            B,
-            next_tokens.data_ptr(),
-            None if logits is None else logits.data_ptr(),
-            1 if use_graph else 0,
-            self.stream.cuda_stream,
-        )
+        captured = self._take(tokens, ctx_lens, block_table, next_tokens, logits)
+        try:
+            call(
+                "b2d_decoder_step",
+                self._h,
+                tokens.data_ptr(),
+                ctx_lens.data_ptr(),
+                block_table.data_ptr(),
+                B,
+                next_tokens.data_ptr(),
+                None if logits is None else logits.data_ptr(),
+                1 if use_graph and captured is None else 0,  # a capture takes no other one
+                self.stream.cuda_stream,
+            )
+        finally:
+            self._give(captured)
         return next_tokens
 
     def generate(
@@ -311,20 +324,25 @@ class DecodeEngine:
             ring = torch.zeros(max(n_steps, 1), B, dtype=torch.int32, device=tokens.device)
         if ring_count is None:
             ring_count = torch.zeros(1, dtype=torch.int32, device=tokens.device)
-        self._take(tokens, ctx_lens, block_table, ring, ring_count)
-        call(
-            "b2d_decoder_generate",
-            self._h,
-            tokens.data_ptr(),
-            ctx_lens.data_ptr(),
-            block_table.data_ptr(),
-            B,
-            n_steps,
-            ring.data_ptr(),
-            ring.shape[0],
-            ring_count.data_ptr(),
-            self.stream.cuda_stream,
-        )
+        captured = self._take(tokens, ctx_lens, block_table, ring, ring_count)
+        try:
+            if captured is not None:
+                raise ValueError("generate replays a graph of its own: capture step() instead")
+            call(
+                "b2d_decoder_generate",
+                self._h,
+                tokens.data_ptr(),
+                ctx_lens.data_ptr(),
+                block_table.data_ptr(),
+                B,
+                n_steps,
+                ring.data_ptr(),
+                ring.shape[0],
+                ring_count.data_ptr(),
+                self.stream.cuda_stream,
+            )
+        finally:
+            self._give(captured)
         return ring
 
     def prefill(
@@ -350,18 +368,21 @@ class DecodeEngine:
             next_token = torch.empty(1, dtype=torch.int32, device=tokens.device)
         if logits is not None and (logits.dtype != torch.float32 or logits.numel() < self.lm_rows):
             raise ValueError(f"logits must be fp32 with >= {self.lm_rows} elements")
-        self._take(tokens, seq_table, next_token, logits)
-        call(
-            "b2d_decoder_prefill",
-            self._h,
-            tokens.data_ptr(),
-            n,
-            seq_table.data_ptr(),
-            start_pos,
-            next_token.data_ptr(),
-            None if logits is None else logits.data_ptr(),
-            self.stream.cuda_stream,
-        )
+        captured = self._take(tokens, seq_table, next_token, logits)
+        try:
+            call(
+                "b2d_decoder_prefill",
+                self._h,
+                tokens.data_ptr(),
+                n,
+                seq_table.data_ptr(),
+                start_pos,
+                next_token.data_ptr(),
+                None if logits is None else logits.data_ptr(),
+                self.stream.cuda_stream,
+            )
+        finally:
+            self._give(captured)
         return next_token
 
     def peer_collectives(self) -> bool:
