@@ -10,17 +10,20 @@
 //
 // The T_b * G query rows of one KV head (G = heads per KV head) are the M side of two tensor-core
 // products per key tile.  head_dim 64 and 128 run on tcgen05 (tree_attn_t5.cuh: 128 or 256 rows
-// share each read of the cache); head_dim 256, whose output rows and tiles do not fit that
-// kernel's TMEM and shared memory, runs on the kernel of this file:
+// share each read of the cache); at head_dim 256 that kernel's two output tiles and two score tiles
+// of 128 rows are 768 columns of TMEM, which has 512 (one output tile of 256 columns with 64-key tiles
+// would fit; it is not built), so it runs on the kernel of this file:
 //  * one CTA per (chunk of keys, 64-row tile of a KV head, sequence): four consumer warps of 16
 //    rows each and one producer warp that streams key tiles (64 keys = 4 pages, TMA, 128-byte
 //    swizzle) through a shared-memory ring;
 //  * S = Q K^T and O += P V on mma.sync m16n8k16, running maximum and sum in registers;
 //  * a sequence cut into several chunks leaves (max, sum, unnormalized output) per row and chunk
 //    in the workspace and a second kernel joins them.
-// Measured for 8 trees of 64 nodes over 8k-32k places at head_dim 128: 874 us on mma.sync, 197 us
+// Measured for 8 trees of 64 nodes over 8k-32k places at head_dim 128: 874 us on mma.sync, 205 us
 // on tcgen05; for one draft of 8 rows over 1021 places 43.7 and 16 us.  So every size goes to
-// tcgen05 where it can.
+// tcgen05 where it can.  At head_dim 256 (8 heads on one KV head, 8 trees of 61-64 nodes over 4k-8k
+// places, 25 GFLOP) this kernel takes 155 us in fp16, 210 us in fp32, 64 us in fp16 with a window of
+// 512: bound by its four MMA warps per SM.
 //
 // fp32 q (or an output wider than fp16) carries q and the weights as hi + lo fp16 pairs, as the decode
 // attention does: two MMAs for one.  A pair has 22 bits down to 2^-14 and no step below 2^-24, so the
