@@ -400,8 +400,10 @@ B2D_API int b2d_qk_norm_rope_append(const void* qkv, int qkv_dtype, int ldqkv,
  * the rows up to itself.  window > 0 further hides every place whose position is <= the row's
  * position - window: positions are the places themselves, except that with a mask the step's own
  * rows have positions[row] (required then; b2d_paged_plan's: row i's is held to ctx_lens[b] ..
- * ctx_lens[b] + i).  A row that sees nothing gives zeros.  What a hidden place holds (infinities
- * and NaN included) changes nothing.
+ * ctx_lens[b] + i).  A row that sees nothing, or scores of -infinity only, gives zeros.  What a
+ * hidden place holds (infinities and NaN included) changes nothing.  A seen v that is not finite
+ * makes its elements of the output infinite or NaN (which of them is open), unless its weight
+ * vanished.
  * out [rows, Hq * HD] (F32, F16 or F16X2 with its lo plane at out + rows * ldout).  Rows
  * of out may lie between rows of q, but share no memory with any (B2D_ERR_UNSUPPORTED).
  * fp16 q with an fp16 output multiplies in fp16 with fp32 sums; every other combination carries q
